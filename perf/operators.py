@@ -11,8 +11,9 @@ Three operators, over the sizes of this repository's own configurations (`convne
 The 8-bit moments. A parameter's elements are cut into blocks of 256 in storage order; each tensor starts a block of its own. Per block
   exp_avg     m = s_m * k|k| / 127^2,  k in -127..127,  s_m = max|m| of the block,  k = sign(m) * round(127 * sqrt(|m| / s_m))
   exp_avg_sq  v = s_v * (k / 255)^4,   k in 0..255,     s_v = max v of the block,   k = round(255 * (v / s_v)^(1/4)), at least 1 where v > 0
-rounded half up from the 64-bit value (a border is decided on more bits than 32), s_m and s_v rounded to fp32. The parameter's own update
-uses the moments before they are rounded to codes.
+rounded half up from the 64-bit value (a border is decided on more bits than 32), s_m and s_v rounded to fp32. The moments are formed in 64 bits, every
+product and sum rounded on its own: (9 s + g) / 10 is often an exact tie between two fp32 scales. The parameter's own update uses the moments before
+they are rounded to codes.
 """
 import math
 import random
@@ -126,7 +127,7 @@ def _to_codes(m, v):
 
 def _from_codes(km, kv, sm, sv):
     k, l = km.double(), kv.double()
-    return k * k.abs() * (sm.double() / 127.0 ** 2)[:, None], (l * l).square() * (sv.double() / 255.0 ** 4)[:, None]
+    return k * k.abs() * (sm.double() * (1.0 / 127.0 ** 2))[:, None], (l * l).square() * (sv.double() * (1.0 / 255.0 ** 4))[:, None]
 
 
 def _adamw_inputs(case, seed):
