@@ -566,6 +566,37 @@ int mpmae_adamw(float* p, const float* g, float* m, float* v, const float* hp, f
                 float beta2, float eps, float wd, size_t n, const uint8_t* decay_mask, float* gnorm2,
                 mpmae_stream_t stream);
 int mpmae_sumsq(const float* x, size_t n, float* out, mpmae_stream_t stream);
+/* AdamW over nt SEPARATE tensors at once (torch.optim.AdamW over a parameter list, main_pretrain.py:312-320, and torch's clip_grad_norm_ in the same
+ * call), fp32 / bf16 / fp16 parameters and gradients mixed freely, moments in fp32 (bits = 32) or in 8 bits (bits = 8). Per element, with
+ * coef = min(1, max_norm / (|g| + 1e-6)) over the gradients of ALL tensors (max_norm <= 0: no norm, coef = 1):
+ *   m = b1 m + (1 - b1) coef g;  v = b2 v + (1 - b2) (coef g)^2;  p = p (1 - lr wd) - lr / (1 - b1^t) m / (sqrt(v) / sqrt(1 - b2^t) + eps)
+ * A tensor without a gradient (NULL) is left alone and its step count stands; so does everything when the norm is not finite (norm_skip[1] = 1).
+ * Steps are counted on the device, so a captured call replays as the next step.
+ *   - ptrs (HOST): {parameter, gradient} address of every tensor, passed to the kernels by value; both in the same dense element order;
+ *   - groups (HOST): {lr, beta1, beta2, eps, weight_decay} of every parameter group;
+ *   - tensors (device, MpmaeAdamwTensor[nt]), chunks (device, int pairs {tensor, index} of every 4096-element piece, by tensor), chunk_first (HOST, nt + 1):
+ *     the static description; off is the tensor's first element in the moment buffers, a multiple of 256, so is every buffer's length;
+ *   - bits = 32: m, v fp32. bits = 8: m int8 / v uint8 codes and one fp32 scale per 256 elements (ms, vs): m = ms k|k| / 127^2, v = vs (k / 255)^4.
+ *     Padding behind a tensor must be zero and stays zero;
+ *   - steps (device int[nt]), hyper (device, MPMAE_ADAMW_HYPER_BYTES * nt, scratch), partials (device double[npartials], scratch, used with max_norm;
+ *     MPMAE_ADAMW_NORM_BLOCKS per started 200 tensors suffice), norm_skip (device float[2]: the norm before the clip, 1 if the step was skipped). */
+#define MPMAE_ADAMW_HYPER_BYTES 56
+#define MPMAE_ADAMW_NORM_BLOCKS 1024
+typedef struct MpmaeAdamwTensor {
+  long long n, off;
+  int group, dt;            /* dt: 0 fp32, 1 bf16, 2 fp16 */
+} MpmaeAdamwTensor;
+typedef struct MpmaeAdamwArgs {
+  const MpmaeAdamwTensor* tensors; const int* chunks; const int* chunk_first;
+  int* steps; void* hyper; double* partials; float* norm_skip;
+  void* m; void* v; float* ms; float* vs;
+  double max_norm;
+  int nt, npartials, bits, pad_;
+} MpmaeAdamwArgs;
+int mpmae_adamw_multi(const MpmaeAdamwArgs* args, const void* const* ptrs, const double* groups, int ngroups, mpmae_stream_t stream);
+/* fp32 values of n (a multiple of 256) 8-bit moments */
+int mpmae_adamw_values(const uint8_t* m_codes, const uint8_t* v_codes, const float* ms, const float* vs, float* m, float* v, long long n,
+                       mpmae_stream_t stream);
 /* hyper-parameter hand-over for replayed steps: copies record (*counter % slots) of a pinned,
  * device-visible ring of {lr, 1/(1-beta1^t), 1/sqrt(1-beta2^t), grad_scale} records into hp and
  * increments *counter, in stream order (the host fills slot t % slots before enqueueing step t and

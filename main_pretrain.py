@@ -28,6 +28,7 @@ from mmearth_train_amd import fcmae  # noqa: E402
 from mmearth_train_amd.config import default_args  # noqa: E402
 from mmearth_train_amd.custom_loss import UncertaintyWeightingStrategy  # noqa: E402
 from mmearth_train_amd.engine_pretrain import train_one_epoch  # noqa: E402
+from mmearth_train_amd.optim import AdamW  # noqa: E402
 from mmearth_train_amd.synth import make_inputs  # noqa: E402
 
 
@@ -94,6 +95,9 @@ def get_args_parser():
     p.add_argument("--compute_dtype", default="bf16", choices=["bf16", "f32"])
     p.add_argument("--fast_path", type=str2bool, default=True,
                    help="HIP-graph step runner with fused AdamW and overlapped RCCL all-reduce")
+    p.add_argument("--opt", default="torch", choices=["torch", "adamw", "adamw8bit"],
+                   help="optimizer of --fast_path False: torch.optim.AdamW, or this package's AdamW over many tensors with fp32 / 8-bit moments")
+    p.add_argument("--clip_grad", type=float, default=None, help="global gradient-norm clip of --opt adamw / adamw8bit")
     return p
 
 
@@ -130,6 +134,10 @@ def main(args):
     if args.use_mixed:
         print("--use_mixed: fp16 autocast + GradScaler are replaced by bf16 activations with fp32 master weights "
               "(--compute_dtype bf16, no loss scaling needed)")
+    if args.fast_path and args.opt != "torch":
+        raise ValueError("--opt chooses the optimizer of --fast_path False: the fused step has an AdamW of its own")
+    if args.clip_grad is not None and args.opt == "torch":
+        raise ValueError("--clip_grad needs --fast_path False and --opt adamw or adamw8bit")
     torch.cuda.set_device(device)
     torch.manual_seed(args.seed + rank)
 
@@ -163,7 +171,11 @@ def main(args):
     else:
         # debugging path through torch autograd + torch.optim.AdamW; gradients are averaged across ranks on every
         # update step (engine_pretrain.train_one_epoch) - the reference wraps the model in DDP (main_pretrain.py:306-310)
-        optimizer = torch.optim.AdamW(param_groups_weight_decay(model, args.weight_decay), lr=args.lr, betas=(0.9, 0.95))
+        groups = param_groups_weight_decay(model, args.weight_decay)
+        if args.opt == "torch":
+            optimizer = torch.optim.AdamW(groups, lr=args.lr, betas=(0.9, 0.95))
+        else:
+            optimizer = AdamW(groups, lr=args.lr, betas=(0.9, 0.95), state_bits=8 if args.opt == "adamw8bit" else 32, max_norm=args.clip_grad)
 
     if args.output_dir:
         Path(args.output_dir).mkdir(parents=True, exist_ok=True)

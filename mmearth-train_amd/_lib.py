@@ -154,6 +154,14 @@ class StemFrontArgs(C.Structure):
                 ("track_activity", c_int), ("act_out", c_void_p)]
 
 
+class AdamwArgs(C.Structure):
+    _fields_ = [("tensors", c_void_p), ("chunks", c_void_p), ("chunk_first", c_void_p), ("steps", c_void_p), ("hyper", c_void_p),
+                ("partials", c_void_p), ("norm_skip", c_void_p), ("m", c_void_p), ("v", c_void_p), ("ms", c_void_p), ("vs", c_void_p),
+                ("max_norm", C.c_double), ("nt", c_int), ("npartials", c_int), ("bits", c_int), ("pad_", c_int)]
+
+
+ADAMW_HYPER_BYTES = 56          # MPMAE_ADAMW_HYPER_BYTES
+ADAMW_NORM_BLOCKS = 1024        # MPMAE_ADAMW_NORM_BLOCKS
 OPT = {n: i for i, n in enumerate("DW DWW NT_GLDS64 NT_BK32 NT_GLDS TN CS_SPLIT RSC_PF RSC_N40 RSC_N80 TN3_BLOCKS TNG_BLOCKS FOLD_GROUP RSC_W5 RSC_ATOMIC DET RSC1 RSC1_ATOMIC RSP RSP_NWV RSP_NARROW RSN3 EVX RST_NW NT_RING".split())}      # enum MpmaeOption (include/mpmae_hip.h)
 PRO = dict(NONE=0, LN_AFFINE=1, GRN=2, GRN_BWD=3, DOWN_GATHER=4, ROW_GATHER=5, IM2COL3=6)
 EPI = dict(STORE=0, GELU_SUMSQ=1, RESID=2, DZ_STATS=3, SCATTER_ROWS=4, DOWN_DGRAD=5)
@@ -233,6 +241,8 @@ SYMBOLS = {
                                     c_void_p, c_void_p, c_int, c_int, c_void_p],
     "mpmae_adamw": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_float, c_float, c_float, c_float,
                     c_size_t, c_void_p, c_void_p, c_void_p],
+    "mpmae_adamw_multi": [P(AdamwArgs), c_void_p, c_void_p, c_int, c_void_p],
+    "mpmae_adamw_values": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, C.c_longlong, c_void_p],
     "mpmae_sumsq": [c_void_p, c_size_t, c_void_p, c_void_p],
     "mpmae_ln_fwd_down": [c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_float, c_int, c_int, c_int,
                           c_void_p, c_void_p],

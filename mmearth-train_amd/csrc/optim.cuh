@@ -1,0 +1,328 @@
+// AdamW over many separate parameter tensors (fp32 / bf16 / fp16 each), moments in fp32 or in 8 bits, optional clip by the global gradient norm.
+//
+//   g' = g * min(1, max_norm / (|g| + 1e-6))         |g| over every tensor of the step
+//   m  <- b1 m + (1 - b1) g'      v <- b2 v + (1 - b2) g'^2
+//   p  <- p (1 - lr wd) - lr / (1 - b1^t) * m / (sqrt(v) / sqrt(1 - b2^t) + eps)
+//
+// 8-bit moments: blocks of 256 elements in storage order (a tensor starts a block of its own), per block
+//   m = s_m k|k| / 127^2 (k int8),  v = s_v (k / 255)^4 (k uint8),  s_m = max|m|, s_v = max v (fp32)
+// The square / fourth-power steps keep the relative step of |m| and sqrt(v) small near the top of a block (1.6 % / 0.8 %) and still reach down to
+// 6e-5 / 1.5e-5 of it; a positive v never becomes code 0, so the denominator of the next step cannot vanish while m stays.
+//
+// Everything is bound by memory: 3 * sizeof(p) + 16 bytes per element (fp32 moments), 3 * sizeof(p) + 4 + 1/16 (8 bits).
+#pragma once
+#include "common.cuh"
+
+#define ADAMW_CHUNK 4096      // elements per workgroup of 256 threads
+#define ADAMW_BLOCK 256       // elements per 8-bit block
+#define ADAMW_MAX_PTRS 200    // tensors per launch: their addresses travel in the kernel arguments (16 bytes each, 4 KB at most)
+#define ADAMW_MAX_GROUPS 64   // parameter groups per hyper launch (40 bytes each) and
+#define ADAMW_MAX_HAS 512     // tensors per hyper launch (one bit each: has a gradient)
+
+struct AdamwTensor {          // device table, one per parameter tensor (host mirror: MpmaeAdamwTensor)
+  long long n, off;           // elements; first element in the flat moment buffers (a multiple of ADAMW_BLOCK)
+  int group, dt;              // parameter group; 0 fp32, 1 bf16, 2 fp16
+};
+struct AdamwHyper {           // device table, one per parameter tensor, written by adamw_hyper_kernel for this step
+  double b1, c1, b2, c2, coef;      // c = 1 - b; coef: the clip factor
+  float decay, step, isbc2, eps;
+};
+struct AdamwPtrs {
+  struct { void* p; const void* g; } at[ADAMW_MAX_PTRS];
+  int first;                  // index of the launch's first tensor
+};
+struct AdamwGroups {
+  struct { double lr, b1, b2, eps, wd; } at[ADAMW_MAX_GROUPS];
+  unsigned has[ADAMW_MAX_HAS / 32];
+  int first, count, t0, t1;   // groups [first, first + count), tensors [t0, t1)
+};
+
+// block-uniform fp64 sum in a fixed order (wave butterflies, then the four waves in order)
+__device__ __forceinline__ double adamw_block_sum(double x, double* red) {
+#pragma unroll
+  for (int d = 32; d; d >>= 1) x += __shfl_xor(x, d);
+  const int w = threadIdx.x >> 6, nw = blockDim.x >> 6;
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) red[w] = x;
+  __syncthreads();
+  double s = 0.0;
+  for (int i = 0; i < nw; ++i) s += red[i];
+  return s;
+}
+
+template <typename T> struct AdamwIo;
+template <> struct AdamwIo<float> {
+  static __device__ __forceinline__ float ld(const float* p) { return *p; }
+  static __device__ __forceinline__ void st(float* p, float v) { *p = v; }
+  static __device__ __forceinline__ void ld8v(const float* p, float (&o)[8]) { ld8(p, o); }
+  static __device__ __forceinline__ void st8v(float* p, const float (&o)[8]) { st8(p, o); }
+};
+template <> struct AdamwIo<bf16_t> {
+  static __device__ __forceinline__ float ld(const bf16_t* p) { return bf2f(*p); }
+  static __device__ __forceinline__ void st(bf16_t* p, float v) { *p = f2bf(v); }
+  static __device__ __forceinline__ void ld8v(const bf16_t* p, float (&o)[8]) { ld8(p, o); }
+  static __device__ __forceinline__ void st8v(bf16_t* p, const float (&o)[8]) { st8(p, o); }
+};
+template <> struct AdamwIo<_Float16> {
+  typedef __attribute__((ext_vector_type(8))) _Float16 h8;
+  static __device__ __forceinline__ float ld(const _Float16* p) { return (float)*p; }
+  static __device__ __forceinline__ void st(_Float16* p, float v) { *p = (_Float16)v; }
+  static __device__ __forceinline__ void ld8v(const _Float16* p, float (&o)[8]) {
+    const h8 a = *reinterpret_cast<const h8*>(p);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) o[i] = (float)a[i];
+  }
+  static __device__ __forceinline__ void st8v(_Float16* p, const float (&o)[8]) {
+    h8 a;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) a[i] = (_Float16)o[i];
+    *reinterpret_cast<h8*>(p) = a;
+  }
+};
+// eight consecutive elements, `left` of them inside the tensor (the others read as 0 and are not written); vec: whole and 16-byte aligned
+template <typename T>
+__device__ __forceinline__ void adamw_ld8(const T* p, long long left, bool vec, float (&o)[8]) {
+  if (vec && left >= 8) { AdamwIo<T>::ld8v(p, o); return; }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) o[i] = i < left ? AdamwIo<T>::ld(p + i) : 0.f;
+}
+template <typename T>
+__device__ __forceinline__ void adamw_st8(T* p, long long left, bool vec, const float (&o)[8]) {
+  if (vec && left >= 8) { AdamwIo<T>::st8v(p, o); return; }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) if (i < left) AdamwIo<T>::st(p + i, o[i]);
+}
+
+// ---------------------------------------------------------------------------------
+// Sum of squares of every gradient of the launch, in fp64 (a factor that went into 8-bit codes must not depend on the summation order): workgroup b
+// walks chunks first + b, first + b + gridDim, ...; one partial per workgroup, no atomics.
+// ---------------------------------------------------------------------------------
+template <typename T>
+__device__ __forceinline__ double adamw_sumsq_chunk(const T* g, long long n, long long base) {
+  const bool vec = (((uintptr_t)g) & 15) == 0;
+  double s = 0.0;
+#pragma unroll
+  for (int it = 0; it < ADAMW_CHUNK / 2048; ++it) {
+    const long long i = base + it * 2048 + threadIdx.x * 8;
+    float x[8];
+    adamw_ld8(g + i, n - i, vec, x);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) s += (double)x[e] * (double)x[e];
+  }
+  return s;
+}
+__global__ __launch_bounds__(256) void adamw_norm_kernel(AdamwPtrs ptrs, const AdamwTensor* __restrict__ tensors, const int2* __restrict__ chunks,
+                                                         int nchunks, double* __restrict__ partials) {
+  __shared__ double red[4];
+  double s = 0.0;
+  for (int c = blockIdx.x; c < nchunks; c += gridDim.x) {
+    const int2 ch = chunks[c];
+    const AdamwTensor t = tensors[ch.x];
+    const void* g = ptrs.at[ch.x - ptrs.first].g;
+    if (!g) continue;
+    const long long base = (long long)ch.y * ADAMW_CHUNK;
+    if (t.dt == 0) s += adamw_sumsq_chunk((const float*)g, t.n, base);
+    else if (t.dt == 1) s += adamw_sumsq_chunk((const bf16_t*)g, t.n, base);
+    else s += adamw_sumsq_chunk((const _Float16*)g, t.n, base);
+  }
+  s = adamw_block_sum(s, red);
+  if (threadIdx.x == 0) partials[blockIdx.x] = s;
+}
+
+// ---------------------------------------------------------------------------------
+// One workgroup: folds the norm's partials, decides on a skip (a non-finite norm leaves everything as it was, steps included), counts the steps of the
+// tensors that have a gradient and writes their records. 1 - b^t in fp64: at t = 1 it is a difference of near-equal numbers.
+// ---------------------------------------------------------------------------------
+__global__ __launch_bounds__(256) void adamw_hyper_kernel(AdamwGroups groups, const AdamwTensor* __restrict__ tensors,
+                                                          int* __restrict__ steps, AdamwHyper* __restrict__ hyper,
+                                                          const double* __restrict__ partials, int npartials, double max_norm,
+                                                          float* __restrict__ norm_skip) {
+  __shared__ double red[4];
+  float coef = 1.f;
+  if (npartials > 0) {
+    double s = 0.0;
+    for (int i = threadIdx.x; i < npartials; i += 256) s += partials[i];
+    const double norm = sqrt(adamw_block_sum(s, red));
+    const bool bad = !(norm < (double)INFINITY);
+    if (threadIdx.x == 0) { norm_skip[0] = (float)norm; norm_skip[1] = bad ? 1.f : 0.f; }
+    if (bad) return;
+    coef = (float)fmin(1.0, max_norm / (norm + 1e-6));
+  }
+  for (int i = groups.t0 + threadIdx.x; i < groups.t1; i += 256) {
+    const int g = tensors[i].group - groups.first;
+    if (g < 0 || g >= groups.count || !(groups.has[(i - groups.t0) >> 5] >> ((i - groups.t0) & 31) & 1)) continue;
+    const int t = steps[i] + 1;
+    steps[i] = t;
+    const double b1 = groups.at[g].b1, b2 = groups.at[g].b2, lr = groups.at[g].lr;
+    AdamwHyper h;
+    h.b1 = b1; h.b2 = b2;
+    h.c1 = 1.0 - b1; h.c2 = 1.0 - b2; h.coef = (double)coef;
+    h.decay = (float)(1.0 - lr * groups.at[g].wd);
+    h.step = (float)(lr / (1.0 - pow(b1, (double)t)));
+    h.isbc2 = (float)(1.0 / sqrt(1.0 - pow(b2, (double)t)));
+    h.eps = (float)groups.at[g].eps;
+    hyper[i] = h;
+  }
+}
+
+// ---------------------------------------------------------------------------------
+// fp32 moments
+// ---------------------------------------------------------------------------------
+template <typename T>
+__device__ __forceinline__ void adamw32_chunk(T* __restrict__ p, const T* __restrict__ g, float* __restrict__ m, float* __restrict__ v, long long n,
+                                              long long base, const AdamwHyper& h) {
+  const bool vec = ((((uintptr_t)p) | ((uintptr_t)g)) & 15) == 0;
+  const float b1 = (float)h.b1, c1 = (float)(h.c1 * h.coef), b2 = (float)h.b2, c2 = (float)(h.c2 * h.coef * h.coef);
+#pragma unroll
+  for (int it = 0; it < ADAMW_CHUNK / 2048; ++it) {
+    const long long i = base + it * 2048 + threadIdx.x * 8;
+    if (i >= n) return;
+    float pv[8], gv[8], mv[8], vv[8];
+    adamw_ld8(p + i, n - i, vec, pv);
+    adamw_ld8(g + i, n - i, vec, gv);
+    ld8(m + i, mv);                       // the flat moment buffers are padded to whole blocks: zero behind the tensor, and zero they stay
+    ld8(v + i, vv);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      mv[e] = b1 * mv[e] + c1 * gv[e];
+      vv[e] = b2 * vv[e] + c2 * gv[e] * gv[e];
+      pv[e] = pv[e] * h.decay - h.step * mv[e] / (sqrtf(vv[e]) * h.isbc2 + h.eps);
+    }
+    adamw_st8(p + i, n - i, vec, pv);
+    st8(m + i, mv);
+    st8(v + i, vv);
+  }
+}
+__global__ __launch_bounds__(256) void adamw32_kernel(AdamwPtrs ptrs, const AdamwTensor* __restrict__ tensors, const int2* __restrict__ chunks,
+                                                      const AdamwHyper* __restrict__ hyper, float* __restrict__ m, float* __restrict__ v,
+                                                      const float* __restrict__ norm_skip) {
+  const int2 ch = chunks[blockIdx.x];
+  const AdamwTensor t = tensors[ch.x];
+  void* p = ptrs.at[ch.x - ptrs.first].p;
+  const void* g = ptrs.at[ch.x - ptrs.first].g;
+  if (!g || (norm_skip && norm_skip[1] != 0.f)) return;
+  const AdamwHyper h = hyper[ch.x];
+  const long long base = (long long)ch.y * ADAMW_CHUNK;
+  if (t.dt == 0) adamw32_chunk((float*)p, (const float*)g, m + t.off, v + t.off, t.n, base, h);
+  else if (t.dt == 1) adamw32_chunk((bf16_t*)p, (const bf16_t*)g, m + t.off, v + t.off, t.n, base, h);
+  else adamw32_chunk((_Float16*)p, (const _Float16*)g, m + t.off, v + t.off, t.n, base, h);
+}
+
+// ---------------------------------------------------------------------------------
+// 8-bit moments. A lane holds eight consecutive elements, 32 lanes a block: the block's maxima are five lane exchanges. The moments are formed in fp64
+// (full rate on this machine) and the codes decided on them: the fp32 estimate of a code is exact except next to a border, where the border itself is
+// compared in fp64. Each fp64 operation rounds on its own, in the order of the formula (no contraction): a block's scale is often an exact tie between
+// two fp32 numbers ((9 s + g) / 10), and the scale, and with it every code, must not depend on how a compiler groups the terms.
+// ---------------------------------------------------------------------------------
+__device__ __forceinline__ unsigned adamw_max32(unsigned x) {      // maximum over the 32 lanes of a half wave (bit patterns of non-negative floats)
+#pragma unroll
+  for (int d = 16; d; d >>= 1) x = max(x, (unsigned)__shfl_xor((int)x, d));
+  return x;
+}
+__device__ __forceinline__ int adamw_code_m(double m, float s, bool direct) {       // |code| in 0..127
+  if (direct) return min((int)floor(127.0 * sqrt(fabs(m) / (double)s) + 0.5), 127);
+  const float t = 127.f * sqrtf(fabsf((float)m) / s);
+  const float f = floorf(t), r = t - f;
+  int k = (int)f + (r >= 0.5f ? 1 : 0);
+  if (fabsf(r - 0.5f) < 1e-3f) {
+    const double b = (double)f + 0.5;
+    k = (int)f + (fabs(m) * 16129.0 >= b * b * (double)s ? 1 : 0);
+  }
+  return min(k, 127);
+}
+__device__ __forceinline__ int adamw_code_v(double v, float s, bool direct) {       // 0..255
+  int k;
+  if (direct) k = (int)floor(255.0 * sqrt(sqrt(v / (double)s)) + 0.5);
+  else {
+    const float t = 255.f * sqrtf(sqrtf((float)v / s));
+    const float f = floorf(t), r = t - f;
+    k = (int)f + (r >= 0.5f ? 1 : 0);
+    if (fabsf(r - 0.5f) < 1e-3f) {
+      const double b = (double)f + 0.5, b2 = b * b;
+      k = (int)f + (v * (65025.0 * 65025.0) >= b2 * b2 * (double)s ? 1 : 0);
+    }
+  }
+  return max(min(k, 255), v > 0.0 ? 1 : 0);
+}
+template <typename T>
+__device__ __forceinline__ void adamw8_chunk(T* __restrict__ p, const T* __restrict__ g, uint8_t* __restrict__ mc, uint8_t* __restrict__ vc,
+                                             float* __restrict__ ms, float* __restrict__ vs, long long n, long long base, const AdamwHyper& h) {
+#pragma clang fp contract(off)
+  const bool vec = ((((uintptr_t)p) | ((uintptr_t)g)) & 15) == 0;
+#pragma unroll 1
+  for (int it = 0; it < ADAMW_CHUNK / 2048; ++it) {
+    const long long blk = (base + it * 2048) / ADAMW_BLOCK + (threadIdx.x >> 5);
+    const long long i = blk * ADAMW_BLOCK + (threadIdx.x & 31) * 8;
+    if (blk * ADAMW_BLOCK >= n) return;              // (uniform over the block's 32 lanes)
+    float pv[8], gv[8];
+    adamw_ld8(p + i, n - i, vec, pv);
+    adamw_ld8(g + i, n - i, vec, gv);
+    uint2 mq = *reinterpret_cast<const uint2*>(mc + i), vq = *reinterpret_cast<const uint2*>(vc + i);
+    const double am = (double)ms[blk] * (1.0 / 16129.0), av = (double)vs[blk] * (1.0 / (65025.0 * 65025.0));
+    double m[8], v[8];
+    unsigned mx = 0, vx = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int km = (int)(int8_t)((e < 4 ? mq.x : mq.y) >> (8 * (e & 3)));
+      const unsigned kv = ((e < 4 ? vq.x : vq.y) >> (8 * (e & 3))) & 255u;
+      const double gd = (double)gv[e] * h.coef;
+      m[e] = h.b1 * ((double)(km * abs(km)) * am) + h.c1 * gd;
+      v[e] = h.b2 * ((double)((kv * kv) * (kv * kv)) * av) + h.c2 * gd * gd;
+      mx = max(mx, __float_as_uint(fabsf((float)m[e])));
+      vx = max(vx, __float_as_uint((float)v[e]) & 0x7fffffffu);
+      pv[e] = pv[e] * h.decay - h.step * (float)m[e] / (sqrtf((float)v[e]) * h.isbc2 + h.eps);
+    }
+    adamw_st8(p + i, n - i, vec, pv);
+    mx = adamw_max32(mx);
+    vx = adamw_max32(vx);
+    // a block with a non-finite moment gets a NaN scale (its moments read back as NaN, as fp32 moments would stay); an empty one the scale 0
+    const bool mbad = mx >= 0x7f800000u, vbad = vx >= 0x7f800000u;
+    const float sm = mbad ? NAN : __uint_as_float(mx), sv = vbad ? NAN : __uint_as_float(vx);
+    const bool mdir = sm < 1e-30f, vdir = sv < 1e-30f;
+    mq = make_uint2(0, 0); vq = make_uint2(0, 0);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      int km = 0, kv = 0;
+      if (!mbad && mx) { km = adamw_code_m(m[e], sm, mdir); km = m[e] < 0.0 ? -km : km; }
+      if (!vbad && vx) kv = adamw_code_v(v[e], sv, vdir);
+      if (e < 4) { mq.x |= ((unsigned)km & 255u) << (8 * e); vq.x |= (unsigned)kv << (8 * e); }
+      else { mq.y |= ((unsigned)km & 255u) << (8 * (e - 4)); vq.y |= (unsigned)kv << (8 * (e - 4)); }
+    }
+    *reinterpret_cast<uint2*>(mc + i) = mq;
+    *reinterpret_cast<uint2*>(vc + i) = vq;
+    if ((threadIdx.x & 31) == 0) { ms[blk] = sm; vs[blk] = sv; }
+  }
+}
+__global__ __launch_bounds__(256) void adamw8_kernel(AdamwPtrs ptrs, const AdamwTensor* __restrict__ tensors, const int2* __restrict__ chunks,
+                                                     const AdamwHyper* __restrict__ hyper, uint8_t* __restrict__ m, uint8_t* __restrict__ v,
+                                                     float* __restrict__ ms, float* __restrict__ vs, const float* __restrict__ norm_skip) {
+  const int2 ch = chunks[blockIdx.x];
+  const AdamwTensor t = tensors[ch.x];
+  void* p = ptrs.at[ch.x - ptrs.first].p;
+  const void* g = ptrs.at[ch.x - ptrs.first].g;
+  if (!g || (norm_skip && norm_skip[1] != 0.f)) return;
+  const AdamwHyper h = hyper[ch.x];
+  const long long base = (long long)ch.y * ADAMW_CHUNK, sb = t.off / ADAMW_BLOCK;
+  if (t.dt == 0) adamw8_chunk((float*)p, (const float*)g, m + t.off, v + t.off, ms + sb, vs + sb, t.n, base, h);
+  else if (t.dt == 1) adamw8_chunk((bf16_t*)p, (const bf16_t*)g, m + t.off, v + t.off, ms + sb, vs + sb, t.n, base, h);
+  else adamw8_chunk((_Float16*)p, (const _Float16*)g, m + t.off, v + t.off, ms + sb, vs + sb, t.n, base, h);
+}
+
+// the values the codes stand for, fp32: 2 + 1/32 bytes read and 8 written per element
+__global__ __launch_bounds__(256) void adamw8_values_kernel(const uint8_t* __restrict__ mc, const uint8_t* __restrict__ vc, const float* __restrict__ ms,
+                                                            const float* __restrict__ vs, float* __restrict__ m, float* __restrict__ v, long long n) {
+  const long long i = ((long long)blockIdx.x * 256 + threadIdx.x) * 8;      // n is a multiple of ADAMW_BLOCK
+  if (i >= n) return;
+  const uint2 mq = *reinterpret_cast<const uint2*>(mc + i), vq = *reinterpret_cast<const uint2*>(vc + i);
+  const double am = (double)ms[i / ADAMW_BLOCK] * (1.0 / 16129.0), av = (double)vs[i / ADAMW_BLOCK] * (1.0 / (65025.0 * 65025.0));
+  float mo[8], vo[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const int km = (int)(int8_t)((e < 4 ? mq.x : mq.y) >> (8 * (e & 3)));
+    const unsigned kv = ((e < 4 ? vq.x : vq.y) >> (8 * (e & 3))) & 255u;
+    mo[e] = (float)((double)(km * abs(km)) * am);
+    vo[e] = (float)((double)((kv * kv) * (kv * kv)) * av);
+  }
+  st8(m + i, mo);
+  st8(v + i, vo);
+}

@@ -1,0 +1,447 @@
+"""AdamW over many tensors on the GPU (mmearth_train_amd.optim) against the formulas in 64 bits on the CPU.
+
+Tolerances. u = 2^-24 is half a step of fp32. A 32-bit moment is two products and a sum of fp32-rounded factors: at most 5 roundings of
+|b1 m| + |c1 g| per step, and the last step's error enters the next one scaled by b1 < 1, so `steps * 5 u` of the largest such sum bounds it. The
+parameter adds p * decay (3 roundings of |p|) and the quotient step * m / (sqrt(v) * isbc2 + eps): at most 10 roundings of its own on top of the
+moments' relative errors (that of v halved by the root). A parameter of fewer bits is rounded once per step on both sides: next to a border the two
+round apart, one whole step of its type (eps). Codes and scales of the 8-bit moments are formed in 64 bits on both sides,
+operation by operation, and have to be equal.
+"""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+U = 2.0 ** -24
+BLOCK = 256
+DT = [torch.float32, torch.bfloat16, torch.float16]
+
+
+class Ref:
+    """One tensor of the definition in 64 bits; the parameter is rounded to its type after every step."""
+
+    def __init__(self, p, bits):
+        self.type, self.bits, self.t = p.dtype, bits, 0
+        self.p = p.detach().double().cpu().reshape(-1)
+        self.m, self.v = torch.zeros_like(self.p), torch.zeros_like(self.p)
+        self.tol_m, self.tol_v, self.tol_p = (torch.zeros_like(self.p) for _ in range(3))
+
+    def step(self, g, coef, lr, b1, b2, eps, wd):
+        self.t += 1
+        g = g.detach().double().cpu().reshape(-1) * coef
+        size_m, size_v = b1 * self.m.abs() + (1 - b1) * g.abs(), b2 * self.v + (1 - b2) * g * g
+        m, v = b1 * self.m + (1 - b1) * g, b2 * self.v + (1 - b2) * g * g
+        self.tol_m = b1 * self.tol_m + (0 if self.bits == 8 else 5 * U) * size_m
+        self.tol_v = b2 * self.tol_v + (0 if self.bits == 8 else 6 * U) * size_v
+        denom = v.sqrt() / math.sqrt(1 - b2 ** self.t) + eps
+        step = lr / (1 - b1 ** self.t)
+        up = step * m / denom
+        self.tol_p = self.tol_p + 3 * U * self.p.abs() + step * (self.tol_m + U * m.abs()) / denom + up.abs() * (12 * U + torch.nan_to_num(self.tol_v / v))
+        self.p = (self.p * (1 - lr * wd) - up)
+        self.tol_p = self.tol_p + (U if self.type == torch.float32 else torch.finfo(self.type).eps) * self.p.abs()
+        if self.type == torch.float16:
+            self.tol_p = self.tol_p + 2.0 ** -24           # a whole step among its subnormals
+        self.p = self.p.to(self.type).double()
+        if self.bits == 32:
+            self.m, self.v = m, v
+        else:
+            (self.km, self.sm), (self.kv, self.sv) = codes(m, False), codes(v, True)
+            self.m, self.v = values(self.km, self.sm, False)[:m.numel()], values(self.kv, self.sv, True)[:m.numel()]
+
+
+def codes(x, fourth):
+    n = x.numel()
+    x = torch.cat([x, x.new_zeros(-n % BLOCK)]).reshape(-1, BLOCK).numpy()
+    s = np.abs(x).max(1).astype(np.float32).astype(np.float64)
+    r = np.divide(np.abs(x), s[:, None], out=np.zeros_like(x), where=s[:, None] > 0)
+    k = np.floor(255 * r ** 0.25 + 0.5).clip(0, 255) if fourth else np.floor(127 * r ** 0.5 + 0.5).clip(0, 127) * np.sign(x)
+    if fourth:
+        k = np.where((x > 0) & (s[:, None] > 0), np.maximum(k, 1), k)        # (a block whose scale rounds to 0 holds nothing)
+    return k, s
+
+
+def values(k, s, fourth):
+    x = k ** 4 * (s * (1 / 255 ** 4))[:, None] if fourth else k * np.abs(k) * (s * (1 / 127 ** 2))[:, None]
+    return torch.from_numpy(x.reshape(-1))
+
+
+def params_of(sizes, types, seed, odd=False):
+    gen = torch.Generator("cuda").manual_seed(seed)
+    out = []
+    for i, n in enumerate(sizes):
+        d = types[i % len(types)]
+        room = torch.randn(n + 1, device="cuda", generator=gen)
+        room = (0.1 * room).to(d)
+        out.append(torch.nn.Parameter(room[1:] if odd else room[:n]))         # odd: rows that begin at no vector boundary
+    return out
+
+
+def grads_for(params, seed, odd=False, scale=1.0):
+    gen = torch.Generator("cuda").manual_seed(seed)
+    for p in params:
+        room = torch.randn(p.numel() + 1, device="cuda", generator=gen) * torch.exp(torch.randn(p.numel() + 1, device="cuda", generator=gen))
+        room = (scale * 0.02 * room).to(p.dtype)
+        p.grad = (room[1:] if odd else room[:p.numel()]).view(p.shape)
+
+
+def check(opt, params, refs, bits):
+    m, v = (x.cpu().double() for x in opt.flat_moments())
+    for p, o, r in zip(params, opt.offsets, refs):
+        n = p.numel()
+        dp = (p.detach().double().cpu().reshape(-1) - r.p).abs()
+        assert bool((dp <= r.tol_p).all()), (n, p.dtype, float((dp - r.tol_p).max()))
+        if bits == 8:
+            plan = opt.plan
+            nb = -(-n // BLOCK)
+            assert torch.equal(plan.m[o:o + nb * BLOCK].cpu().double(), torch.from_numpy(r.km.reshape(-1))), (n, p.dtype)
+            assert torch.equal(plan.v[o:o + nb * BLOCK].cpu().double(), torch.from_numpy(r.kv.reshape(-1))), (n, p.dtype)
+            assert torch.equal(plan.ms[o // BLOCK:o // BLOCK + nb].cpu().double(), torch.from_numpy(r.sm))
+            assert torch.equal(plan.vs[o // BLOCK:o // BLOCK + nb].cpu().double(), torch.from_numpy(r.sv))
+            # read back in fp32: one rounding of the value, half a step: 2^-24 of it, or 2^-150 where it is subnormal (those are 2^-149 apart)
+            assert bool(((m[o:o + n] - r.m).abs() <= 1.01 * U * r.m.abs() + 2.0 ** -150).all())
+            assert bool(((v[o:o + n] - r.v).abs() <= 1.01 * U * r.v.abs() + 2.0 ** -150).all())
+        else:
+            assert bool(((m[o:o + n] - r.m).abs() <= r.tol_m + 1e-45).all()), (n, p.dtype)
+            assert bool(((v[o:o + n] - r.v).abs() <= r.tol_v + 1e-45).all()), (n, p.dtype)
+        assert not m[o + n:o + -(-n // BLOCK) * BLOCK].any() and not v[o + n:o + -(-n // BLOCK) * BLOCK].any()
+
+
+def run_steps(opt, params, refs, steps, clip=None, odd=False, lacking=()):
+    for k in range(steps):
+        grads_for(params, 100 + k, odd, scale=10.0 if k == 1 else 1.0)
+        for i in lacking:
+            if (i + k) % 2 == 0:
+                params[i].grad = None
+        before = [p.grad.clone() for p in params if p.grad is not None]
+        coef = 1.0
+        if clip:
+            norm = math.sqrt(sum(float(p.grad.double().square().sum()) for p in params if p.grad is not None))
+            coef = float(np.float32(min(1.0, clip / (norm + 1e-6))))
+        opt.step()
+        if clip:
+            assert abs(float(opt.grad_norm) - norm) <= 2 * U * norm
+        assert all(torch.equal(a, b) for a, b in zip(before, (p.grad for p in params if p.grad is not None)))
+        i = 0
+        for g in opt.param_groups:
+            for p in g["params"]:
+                if p.grad is not None:
+                    refs[i].step(p.grad, coef, g["lr"], *g["betas"], g["eps"], g["weight_decay"])
+                i += 1
+
+
+SIZES = [1, 7, 255, 256, 257, 2047, 4096, 4097, 10007, 3, 65536 + 13]
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("types", [DT[:1], DT[1:2], DT[2:], DT], ids=["fp32", "bf16", "fp16", "mixed"])
+@pytest.mark.parametrize("odd", [False, True], ids=["aligned", "odd"])
+def test_steps_match_the_definition(bits, types, odd):
+    from mmearth_train_amd.optim import AdamW
+    params = params_of(SIZES, types, 3, odd)
+    refs = [Ref(p, bits) for p in params]
+    opt = AdamW([{"params": params[:4], "weight_decay": 0.0}, {"params": params[4:], "betas": (0.8, 0.999), "lr": 3e-3}], lr=1e-3, betas=(0.9, 0.95),
+                weight_decay=0.05, state_bits=bits)
+    run_steps(opt, params, refs, 4, odd=odd, lacking=(2, 5))
+    check(opt, params, refs, bits)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("clip", [0.05, 1e4])
+def test_clip_uses_the_norm_of_every_gradient(bits, clip):
+    from mmearth_train_amd.optim import AdamW
+    params = params_of(SIZES, DT, 4)
+    refs = [Ref(p, bits) for p in params]
+    opt = AdamW(params, lr=1e-3, state_bits=bits, max_norm=clip)
+    run_steps(opt, params, refs, 3, clip=clip, lacking=(1,))
+    assert float(opt.skipped) == 0.0
+    check(opt, params, refs, bits)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_more_tensors_and_groups_than_one_launch_takes(bits):
+    from mmearth_train_amd.optim import AdamW
+    sizes = [1 + (i * 37) % 700 for i in range(1100)]
+    params = params_of(sizes, DT, 5)
+    refs = [Ref(p, bits) for p in params]
+    opt = AdamW([{"params": params[i:i + 8], "lr": 1e-3 * (1 + i / 100), "weight_decay": 0.01 * (i % 3)} for i in range(0, 1100, 8)], state_bits=bits,
+                max_norm=0.5)
+    run_steps(opt, params, refs, 2, clip=0.5)
+    check(opt, params, refs, bits)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_norm_that_is_not_finite_changes_nothing(bits):
+    from mmearth_train_amd.optim import AdamW
+    params = params_of([300, 5000], DT[:2], 6)
+    opt = AdamW(params, state_bits=bits, max_norm=1.0)
+    grads_for(params, 1)
+    opt.step()
+    keep = [p.detach().clone() for p in params], [x.clone() for x in opt.flat_moments()], opt.plan.steps.clone()
+    for bad in (float("inf"), float("nan"), -float("inf")):
+        grads_for(params, 2)
+        params[1].grad[4321] = bad
+        opt.step()
+        assert float(opt.skipped) == 1.0 and not math.isfinite(float(opt.grad_norm))
+        assert all(torch.equal(a, b.detach()) for a, b in zip(keep[0], params))
+        assert all(torch.equal(a, b) for a, b in zip(keep[1], opt.flat_moments()))
+        assert torch.equal(keep[2], opt.plan.steps)
+    grads_for(params, 3)
+    opt.step()
+    assert float(opt.skipped) == 0.0 and opt.plan.steps.tolist() == [2, 2]
+
+
+def test_without_a_clip_a_bad_gradient_stays_in_its_block():
+    from mmearth_train_amd.optim import AdamW
+    params = params_of([1024], DT[:1], 7)
+    opt = AdamW(params, state_bits=8)
+    grads_for(params, 1)
+    params[0].grad[300] = float("nan")
+    opt.step()
+    m, v = opt.flat_moments()
+    bad = torch.zeros(1024, dtype=torch.bool, device="cuda")
+    bad[256:512] = True
+    assert torch.equal(torch.isnan(m), bad) and torch.equal(torch.isnan(v), bad)
+    assert torch.isnan(params[0]).nonzero().flatten().tolist() == [300]
+
+
+def test_tiny_and_zero_gradients():
+    """Blocks whose scale is far below fp32's normal range, or nothing at all."""
+    from mmearth_train_amd.optim import AdamW
+    params = params_of([256 * 6], DT[:1], 8)
+    refs = [Ref(params[0], 8)]
+    opt = AdamW(params, state_bits=8, eps=1e-8)
+    for k in range(3):
+        grads_for(params, 20 + k)
+        g = params[0].grad.view(6, 256)
+        g[0] = 0.0
+        g[1] *= 1e-18              # v near 1e-39: subnormal scale
+        g[2] *= 1e-30              # v under every fp32 number, m still normal
+        g[3, 1:] = 0.0
+        g[4, ::2] *= 1e-12
+        opt.step()
+        refs[0].step(params[0].grad, 1.0, 1e-3, 0.9, 0.999, 1e-8, 1e-2)
+    check(opt, params, refs, 8)
+
+
+def test_other_element_orders():
+    """Parameters that are dense in another order than row-major, gradients in a third one."""
+    from mmearth_train_amd.optim import AdamW
+    for bits in (32, 8):
+        gen = torch.Generator("cuda").manual_seed(9)
+        w = torch.nn.Parameter(torch.randn(8, 12, 5, 5, device="cuda", generator=gen).contiguous(memory_format=torch.channels_last))
+        q = torch.nn.Parameter(torch.randn(40, 30, device="cuda", generator=gen).t())
+        g, h = torch.randn(8, 12, 5, 5, device="cuda", generator=gen), torch.randn(30, 40, device="cuda", generator=gen)
+        w.grad, q.grad = g.clone(), h.clone()
+        a = torch.nn.Parameter(w.detach().clone().contiguous())
+        b = torch.nn.Parameter(q.detach().clone().contiguous())
+        a.grad, b.grad = g.clone(), h.clone()
+        one, two = AdamW([w, q], state_bits=32), AdamW([a, b], state_bits=32)
+        for _ in range(2):
+            one.step()
+            two.step()
+        assert torch.equal(w, a) and torch.equal(q, b)
+        s, t = one.state_dict()["state"], two.state_dict()["state"]
+        assert all(torch.equal(s[i][k], t[i][k]) for i in (0, 1) for k in ("exp_avg", "exp_avg_sq"))
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_checkpoints_go_both_ways_with_torch(bits):
+    from mmearth_train_amd.optim import AdamW
+    params = params_of([33, 4500, 257], DT[:1], 10)
+    mine = AdamW(params, lr=2e-3, betas=(0.9, 0.95), weight_decay=0.05, state_bits=bits)
+    for k in range(3):
+        grads_for(params, 30 + k)
+        mine.step()
+    sd = mine.state_dict()
+    theirs = torch.optim.AdamW([torch.nn.Parameter(p.detach().clone()) for p in params], lr=1.0)
+    theirs.load_state_dict(sd)
+    assert theirs.param_groups[0]["lr"] == 2e-3
+    again = AdamW([torch.nn.Parameter(p.detach().clone()) for p in params], lr=1.0, state_bits=bits)
+    again.load_state_dict(theirs.state_dict())
+    assert all(torch.equal(a, b) for a, b in zip(mine.flat_moments(), again.flat_moments()))
+    if bits == 8:
+        assert torch.equal(mine.plan.m, again.plan.m) and torch.equal(mine.plan.v, again.plan.v)
+    grads_for(params, 40)
+    for p, q, r in zip(params, theirs.param_groups[0]["params"], again.param_groups[0]["params"]):
+        q.grad, r.grad = p.grad.clone(), p.grad.clone()
+    mine.step(), theirs.step(), again.step()
+    for p, q, r in zip(params, theirs.param_groups[0]["params"], again.param_groups[0]["params"]):
+        assert torch.equal(p, r)
+        # both round p * decay and the update of at most lr * sqrt(10) or so a few times: 16 roundings of |p| + 0.01 leave room for either order
+        assert bool(((p - q).abs() <= 16 * U * (p.abs() + 0.01)).all())
+
+
+def test_a_captured_step_replays_as_the_next_one():
+    from mmearth_train_amd.optim import AdamW
+    for bits in (32, 8):
+        params, eager = params_of([700, 9000], DT[:2], 11), params_of([700, 9000], DT[:2], 11)
+        a, b = (AdamW(ps, lr=1e-3, state_bits=bits, max_norm=0.7) for ps in (params, eager))
+        for ps in (params, eager):
+            grads_for(ps, 50)
+        a.step(), b.step()
+        graph = torch.cuda.CUDAGraph()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph):
+            a.step()
+        for k in range(4):
+            for p, q in zip(params, eager):
+                q.grad.normal_(generator=torch.Generator("cuda").manual_seed(60 + k))
+                p.grad.copy_(q.grad)
+            graph.replay()
+            b.step()
+            torch.cuda.synchronize()
+            assert torch.equal(a.plan.steps, b.plan.steps)
+            assert all(torch.equal(p, q) for p, q in zip(params, eager))
+            assert all(torch.equal(x, y) for x, y in zip(a.flat_moments(), b.flat_moments()))
+            torch.zeros(1 << 20, device="cuda").sum().item()
+
+
+def test_state_must_exist_before_a_capture():
+    from mmearth_train_amd.optim import AdamW
+    params = params_of([10], DT[:1], 12)
+    grads_for(params, 1)
+    opt = AdamW(params)
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="eager step"):
+        with torch.cuda.graph(graph):
+            opt.step()
+
+
+def test_own_stream_and_determinism():
+    from mmearth_train_amd.optim import AdamW
+    got = []
+    for k in range(2):
+        params = params_of(SIZES, DT, 13)
+        opt = AdamW(params, state_bits=8, max_norm=0.1)
+        s = torch.cuda.Stream()
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            for i in range(3):
+                grads_for(params, 70 + i)
+                opt.step()
+        torch.cuda.current_stream().wait_stream(s)
+        got.append([p.detach().clone() for p in params] + list(opt.flat_moments()) + [opt.grad_norm.clone()])
+    assert all(torch.equal(a, b) for a, b in zip(*got))
+
+
+def test_groups_added_later_and_schedulers():
+    from mmearth_train_amd.optim import AdamW
+    params = params_of([500, 300, 1000], DT[:1], 14)
+    refs = [Ref(p, 32) for p in params]
+    opt = AdamW(params[:2], lr=1e-3)
+    sched = torch.optim.lr_scheduler.StepLR(opt, 1, 0.5)
+    run_steps(opt, params[:2], refs, 2)
+    sched.step()
+    assert opt.param_groups[0]["lr"] == 5e-4
+    opt.add_param_group({"params": [params[2]], "lr": 1e-2})
+    run_steps(opt, params, refs, 2)
+    check(opt, params, refs, 32)
+    assert opt.plan.steps.tolist() == [4, 4, 2]
+
+
+def test_refusals_on_the_device():
+    from mmearth_train_amd.optim import AdamW
+    x = torch.zeros(64, device="cuda")
+    mk = torch.nn.Parameter
+    with pytest.raises(ValueError, match="share memory"):
+        AdamW([mk(x[:40]), mk(x[30:])])
+    with pytest.raises(ValueError, match="densely"):
+        AdamW([mk(x[::2])])
+    with pytest.raises(ValueError, match="twice"):
+        p = mk(x)
+        AdamW([p, p])
+    p = mk(torch.zeros(8, device="cuda"))
+    opt = AdamW([p, mk(torch.zeros(0, device="cuda"))])
+    opt.step()                                          # no gradient anywhere: nothing happens
+    assert opt.state_dict()["state"] == {}
+    p.grad = torch.ones(8, device="cuda")
+    opt.step()
+    p.data = torch.zeros(9, device="cuda")
+    p.grad = None
+    with pytest.raises(ValueError, match="another size"):
+        opt.step()
+    with pytest.raises(RuntimeError, match="max_norm"):
+        opt.grad_norm
+    with pytest.raises(TypeError, match="state_dict"):
+        import copy
+        copy.deepcopy(opt)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_tensor_longer_than_31_bits(bits):
+    """Element offsets past 2^31: the last elements against a small tensor that holds the same values in the same block places."""
+    from mmearth_train_amd.optim import AdamW
+    n, tail = 2 ** 31 + 5003, 5003 + 256
+    p = torch.nn.Parameter(torch.zeros(n, dtype=torch.bfloat16, device="cuda"))
+    p.grad = torch.zeros(n, dtype=torch.bfloat16, device="cuda")
+    start = 2 ** 31 - 256
+    small = params_of([tail], DT[1:2], 15)
+    grads_for(small, 16)
+    p.data[start:] = small[0].data
+    p.grad[start:] = small[0].grad
+    a, b = AdamW([p], state_bits=bits, max_norm=0.5), AdamW(small, state_bits=bits, max_norm=0.5)
+    for _ in range(2):
+        a.step()
+        b.step()
+    assert torch.equal(a.grad_norm, b.grad_norm)
+    assert torch.equal(p.data[start:], small[0].data) and not bool(p.data[:start].any())
+    if bits == 8:
+        assert torch.equal(a.plan.m[start:start + tail], b.plan.m[:tail]) and torch.equal(a.plan.v[start:start + tail], b.plan.v[:tail])
+    else:
+        assert torch.equal(a.plan.m[start:start + tail], b.plan.m[:tail]) and torch.equal(a.plan.v[start:start + tail], b.plan.v[:tail])
+
+
+def test_autograd_notices_the_update():
+    """A step between forward and backward of a graph that saved the parameter is an error, as with torch's own optimizers."""
+    from mmearth_train_amd.optim import AdamW
+    w = torch.nn.Parameter(torch.randn(4, 4, device="cuda"))
+    x = torch.randn(4, 4, device="cuda", requires_grad=True)
+    w.grad = torch.ones_like(w)
+    y = (x @ w).sum()
+    AdamW([w]).step()
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+
+
+def test_a_step_beside_a_live_graph_of_the_same_leaves():
+    """Backward under capture while an eager graph of the same parameters is alive is not this optimizer's business; its own capture is."""
+    from mmearth_train_amd.optim import AdamW
+    w = torch.nn.Parameter(torch.randn(64, 64, device="cuda"))
+    opt = AdamW([w], lr=1e-2)
+    (w * w).sum().backward()
+    opt.step()
+    alive = (w * w).sum()                    # an eager graph over w that nothing ever runs backward
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opt.step()
+    before = w.detach().clone()
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+    assert not torch.equal(before, w) and opt.plan.steps.tolist() == [4] and alive.requires_grad
+
+
+@pytest.mark.parametrize("opt", ["adamw", "adamw8bit"])
+def test_main_pretrain_trains_and_resumes_with_it(opt, tmp_path):
+    """--fast_path False --opt adamw / adamw8bit --clip_grad: two epochs, the second one resumed from the first one's checkpoint."""
+    import main_pretrain
+    common = ["--model", "convnextv2_atto", "--input_size", "56", "--patch_size", "8", "--batch_size", "2", "--update_freq", "2", "--steps_per_epoch", "4",
+              "--lr", "1e-3", "--norm_pix_loss", "True", "--fast_path", "False", "--out_modalities", "pix_mod", "--opt", opt, "--clip_grad", "1.0",
+              "--warmup_epochs", "0", "--output_dir", str(tmp_path)]
+    for epochs in ("1", "2"):
+        stats = main_pretrain.main(main_pretrain.get_args_parser().parse_args(common + ["--epochs", epochs]))
+        assert math.isfinite(stats[0]["loss"])
+    ck = [torch.load(tmp_path / f"checkpoint-{i}.pth", map_location="cpu", weights_only=False) for i in (0, 1)]
+    assert [float(c["optimizer"]["state"][0]["step"]) for c in ck] == [2.0, 4.0]
+    assert not torch.equal(ck[0]["model"]["proj.weight"], ck[1]["model"]["proj.weight"])
+
+
+def test_main_pretrain_refuses_settings_that_would_do_nothing():
+    import main_pretrain
+    base = ["--model", "convnextv2_atto", "--input_size", "56", "--patch_size", "8"]
+    for extra in (["--opt", "adamw"], ["--clip_grad", "1.0"], ["--fast_path", "False", "--clip_grad", "1.0"]):
+        with pytest.raises(ValueError, match="--opt|--clip_grad"):
+            main_pretrain.main(main_pretrain.get_args_parser().parse_args(base + extra))
