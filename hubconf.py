@@ -18,6 +18,7 @@ if ROOT not in sys.path:
 
 from mmearth_train_amd import convnextv2  # noqa: E402
 from mmearth_train_amd.helpers import load_state_dict, remap_checkpoint_keys  # noqa: E402
+from mmearth_train_amd.int8 import quantize_model  # noqa: E402
 
 dependencies = ["torch"]
 
@@ -49,7 +50,8 @@ def load_custom_checkpoint(model, checkpoint, linear_probe):
 
 
 def MPMAE(model_name="convnextv2_atto", ckpt_name="pt-all_mod_atto_1M_64_uncertainty_56-8", pretrained=True,
-          linear_probe=True, **kwargs):
+          linear_probe=True, int8=False, **kwargs):
+    """int8=True: the model is moved to the current GPU and its linear layers are served in 8-bit integers (inference only)."""
     model = convnextv2.__dict__[model_name](**kwargs)
     if pretrained:
         if ckpt_name in CKPT_URLS:
@@ -60,4 +62,4 @@ def MPMAE(model_name="convnextv2_atto", ckpt_name="pt-all_mod_atto_1M_64_uncerta
                 raise ValueError(f"unknown checkpoint {ckpt_name!r}: not a released name {sorted(CKPT_URLS)} nor a file")
             checkpoint = torch.load(path, map_location="cpu", weights_only=False)
         model = load_custom_checkpoint(model, checkpoint, linear_probe)
-    return model
+    return quantize_model(model.cuda().eval()) if int8 else model

@@ -370,6 +370,20 @@ int mpmae_quant_mx(const void* x_bf16, int ld, int rows, int K, void* q, uint32_
 int mpmae_gemm_mx(int epi, const MpmaeGemmArgs* args, const uint32_t* scales_a, int lsa, const uint32_t* scales_b, int lsb,
                   mpmae_stream_t stream);
 
+/* ---- 8-bit integer linear layer (inference of nn.Linear: pwconv1 / pwconv2 / head of the dense network, convnextv2.py:46-52) ----------------
+ * mpmae_quant_i8: M rows of K elements (dt: 0 fp32, 1 bf16, 2 fp16; ldx elements from row to row) to int8 codes q[M][ldq] and scale[M]:
+ *   scale = max|x| / 127, q = round(127 x / max|x|), half to even; a row with NaN or infinity: scale NaN, codes 0. ldq: a multiple of 128, zeros from K on.
+ * mpmae_linear_i8: y[M][N] = sx[m] sw[n] (q w^T)[m][n] + bias[n] (bias may be NULL, fp32), y in x's type: quantises the rows of x into the workspace
+ *   q[M][ldq], sx[M] and multiplies them with w[N][ldw] (from mpmae_quant_i8; ldw == ldq); exact 32-bit integer sums (K <= 131071). q, w 16-byte aligned. */
+typedef struct MpmaeI8Args {
+  const void* x; int8_t* q; float* sx;
+  const int8_t* w; const float* sw; const float* bias; void* y;
+  long long ldx, ldy;
+  int M, N, K, ldq, ldw, pad_;
+} MpmaeI8Args;
+int mpmae_quant_i8(int dt, const void* x, long long ldx, int M, int K, int8_t* q, int ldq, float* scale, mpmae_stream_t stream);
+int mpmae_linear_i8(int dt, const MpmaeI8Args* args, mpmae_stream_t stream);
+
 /* ---- library options ------------------------------------------------------------------------
  * Process-wide kernel-selection / launch-shape switches for A/B measurements (set them before recording launch programs:
  * a recorded launch keeps the choice it was recorded with). The library reads NO environment variables; this table and

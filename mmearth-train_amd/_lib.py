@@ -160,6 +160,13 @@ class AdamwArgs(C.Structure):
                 ("max_norm", C.c_double), ("nt", c_int), ("npartials", c_int), ("bits", c_int), ("pad_", c_int)]
 
 
+class I8Args(C.Structure):
+    _fields_ = [("x", c_void_p), ("q", c_void_p), ("sx", c_void_p), ("w", c_void_p), ("sw", c_void_p), ("bias", c_void_p), ("y", c_void_p),
+                ("ldx", C.c_longlong), ("ldy", C.c_longlong),
+                ("M", c_int), ("N", c_int), ("K", c_int), ("ldq", c_int), ("ldw", c_int), ("pad_", c_int)]
+
+
+I8_KPAD = 128                   # rows of int8 codes are padded to a multiple of this
 ADAMW_HYPER_BYTES = 56          # MPMAE_ADAMW_HYPER_BYTES
 ADAMW_NORM_BLOCKS = 1024        # MPMAE_ADAMW_NORM_BLOCKS
 OPT = {n: i for i, n in enumerate("DW DWW NT_GLDS64 NT_BK32 NT_GLDS TN CS_SPLIT RSC_PF RSC_N40 RSC_N80 TN3_BLOCKS TNG_BLOCKS FOLD_GROUP RSC_W5 RSC_ATOMIC DET RSC1 RSC1_ATOMIC RSP RSP_NWV RSP_NARROW RSN3 EVX RST_NW NT_RING".split())}      # enum MpmaeOption (include/mpmae_hip.h)
@@ -243,6 +250,8 @@ SYMBOLS = {
                     c_size_t, c_void_p, c_void_p, c_void_p],
     "mpmae_adamw_multi": [P(AdamwArgs), c_void_p, c_void_p, c_int, c_void_p],
     "mpmae_adamw_values": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, C.c_longlong, c_void_p],
+    "mpmae_quant_i8": [c_int, c_void_p, C.c_longlong, c_int, c_int, c_void_p, c_int, c_void_p, c_void_p],
+    "mpmae_linear_i8": [c_int, P(I8Args), c_void_p],
     "mpmae_sumsq": [c_void_p, c_size_t, c_void_p, c_void_p],
     "mpmae_ln_fwd_down": [c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_float, c_int, c_int, c_int,
                           c_void_p, c_void_p],

@@ -1,0 +1,142 @@
+"""Linear layers in 8-bit integers on MI355X, for serving the dense network (`hubconf.MPMAE(..., int8=True)`): weights quantised once per output
+channel, activations per row (token, pixel) inside the call, exact integer sums on the matrix cores, scales and bias applied on the way out.
+
+    w = quantize_weight(layer.weight, layer.bias)      # once
+    y = linear_int8(x, w)                              # [..., K] fp32 / bf16 / fp16 -> [..., N] of the same type
+    quantize_model(model)                              # every nn.Linear of a module tree, in place
+
+    x_q = round(127 x / max|x|), s_x = max|x| / 127 per row;  y = s_x s_w (x_q w_q^T) + bias
+
+Inference only: an input that requires a gradient is refused. There is no CPU form.
+"""
+import ctypes as C
+
+import torch
+import torch.nn as nn
+
+from . import _lib
+
+_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+MAX_K = 131071          # 127 * 127 * K fits 32 bits
+
+
+def _rows(x, k):
+    """x as rows of k elements that lie next to each other: (tensor that owns them, rows, elements from row to row)."""
+    if x.dim() != 2 or (x.stride(1) != 1 and k > 1):
+        x = x.reshape(-1, k)
+        if x.stride(1) != 1 and k > 1:
+            x = x.contiguous()
+    return x, x.shape[0], x.stride(0)
+
+
+def _stream(device):
+    return torch.cuda.current_stream(device).cuda_stream
+
+
+class Int8Weight:
+    """A weight matrix [N, K] as int8 codes with one scale per row, laid out for `linear_int8`. Made by `quantize_weight`."""
+
+    def __init__(self, q, scale, bias, k):
+        self.q, self.scale, self.bias, self.k, self.n = q, scale, bias, k, q.shape[0]
+        self.device = q.device
+
+    def dequantize(self):
+        """The fp32 matrix that the codes stand for."""
+        return self.q[:, :self.k].float() * self.scale[:, None]
+
+
+@torch.no_grad()
+def quantize_weight(weight, bias=None):
+    """weight [N, K] fp32 / bf16 / fp16 (and bias [N]) of a linear layer on the GPU -> Int8Weight."""
+    if weight.dim() != 2 or 0 in weight.shape:
+        raise ValueError(f"a weight is a matrix [N, K] with at least one element, not {tuple(weight.shape)}")
+    if weight.dtype not in _DTYPES:
+        raise ValueError(f"weights are fp32, bf16 or fp16, not {weight.dtype}")
+    if weight.shape[1] > MAX_K:
+        raise ValueError(f"rows of at most {MAX_K} elements: their integer sums fit 32 bits")
+    if bias is not None and (bias.shape != weight.shape[:1] or bias.dtype not in _DTYPES or bias.device != weight.device):
+        raise ValueError(f"a bias is a floating vector [{weight.shape[0]}] on the weight's device")
+    if weight.device.type != "cuda":
+        raise ValueError(f"this layer runs on the GPU only: the weight is on {weight.device}")
+    n, k = weight.shape
+    w, _, ld = _rows(weight, k)
+    kp = -(-k // _lib.I8_KPAD) * _lib.I8_KPAD
+    q = torch.empty(n, kp, dtype=torch.int8, device=weight.device)
+    scale = torch.empty(n, dtype=torch.float32, device=weight.device)
+    with torch.cuda.device(weight.device):
+        err = _lib.load().mpmae_quant_i8(_DTYPES[w.dtype], w.data_ptr(), ld, n, k, q.data_ptr(), kp, scale.data_ptr(), _stream(weight.device))
+    _lib.check(err, "quant_i8")
+    return Int8Weight(q, scale, None if bias is None else bias.detach().float().contiguous(), k)
+
+
+def linear_int8(x, w):
+    """y = x W^T + bias for x [..., K] fp32 / bf16 / fp16 on the weight's GPU; y has x's type. A row that holds NaN or infinity gives a row of NaN."""
+    if x.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError("linear_int8 has no backward pass: call it under torch.no_grad()")
+    dt = _DTYPES.get(x.dtype)
+    if dt is None:
+        raise ValueError(f"inputs are fp32, bf16 or fp16, not {x.dtype}")
+    if x.dim() < 1 or x.shape[-1] != w.k:
+        raise ValueError(f"inputs end in {w.k} elements, the weight's: got {tuple(x.shape)}")
+    if x.device != w.device:
+        raise ValueError(f"the input is on {x.device}, the weight on {w.device}")
+    y = torch.empty(x.shape[:-1] + (w.n,), dtype=x.dtype, device=x.device)
+    if not y.numel():
+        return y
+    x, m, ld = _rows(x, w.k)
+    kp = w.q.shape[1]
+    ws = torch.empty(m * (kp + 4), dtype=torch.uint8, device=x.device)       # codes, then scales
+    at = ws.data_ptr()
+    args = _lib.I8Args(x.data_ptr(), at, at + m * kp, w.q.data_ptr(), w.scale.data_ptr(), None if w.bias is None else w.bias.data_ptr(), y.data_ptr(),
+                       ld, w.n, m, w.n, w.k, kp, kp, 0)
+    if torch.cuda.current_device() == x.device.index:
+        err = _lib.load().mpmae_linear_i8(dt, C.byref(args), _stream(x.device))
+    else:
+        with torch.cuda.device(x.device):
+            err = _lib.load().mpmae_linear_i8(dt, C.byref(args), _stream(x.device))
+    _lib.check(err, "linear_i8")
+    return y
+
+
+class Int8Linear(nn.Module):
+    """nn.Linear with int8 weights, inference only. Codes, scales and bias are buffers: they are saved, loaded and moved with the model; `.half()` and
+    the like leave them in their own types."""
+
+    def __init__(self, in_features, out_features, bias=True, device=None):
+        super().__init__()
+        self.in_features, self.out_features = in_features, out_features
+        kp = -(-in_features // _lib.I8_KPAD) * _lib.I8_KPAD
+        self.register_buffer("q", torch.zeros(out_features, kp, dtype=torch.int8, device=device))
+        self.register_buffer("scale", torch.zeros(out_features, dtype=torch.float32, device=device))
+        self.register_buffer("bias", torch.zeros(out_features, dtype=torch.float32, device=device) if bias else None)
+
+    @classmethod
+    def from_linear(cls, linear):
+        w = quantize_weight(linear.weight, linear.bias)
+        self = cls(linear.in_features, linear.out_features, linear.bias is not None, device="meta")
+        self.q, self.scale, self.bias = w.q, w.scale, w.bias
+        return self
+
+    def _apply(self, fn, recurse=True):
+        for name, buf in self._buffers.items():
+            if buf is not None:
+                moved = fn(buf)
+                self._buffers[name] = moved if moved.dtype == buf.dtype else buf.to(moved.device)
+        return self
+
+    def forward(self, x):
+        return linear_int8(x, Int8Weight(self.q, self.scale, self.bias, self.in_features))
+
+    def extra_repr(self):
+        return f"in_features={self.in_features}, out_features={self.out_features}, bias={self.bias is not None}"
+
+
+def quantize_model(model):
+    """Every nn.Linear of the module tree (on the GPU) becomes an Int8Linear, in place; returns the model."""
+    if isinstance(model, nn.Linear):
+        return Int8Linear.from_linear(model)
+    for name, child in model.named_children():
+        new = quantize_model(child)
+        if new is not child:
+            setattr(model, name, new)
+    return model

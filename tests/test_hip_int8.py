@@ -1,0 +1,250 @@
+"""The int8 linear layer on the GPU (mmearth_train_amd.int8) against the definition in 64 bits on the CPU.
+
+Tolerances. The codes are whole numbers and equal. y: the exact integer sum is rounded to fp32 (2^-24), multiplied by two scales that are rounded
+to fp32 (2^-24 each, two products: 2^-24 each), added to the bias (2^-24 of the result) and rounded once to the type: at most 6 * 2^-24 of |q-product| and
+of |y| + half a step of the type.
+"""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+U = 2.0 ** -24
+DT = {"fp32": torch.float32, "bf16": torch.bfloat16, "fp16": torch.float16}
+
+
+def ref_codes(x):
+    x = x.detach().double().cpu()
+    a = x.abs().amax(-1)
+    q = torch.round(127.0 * x / torch.where(a == 0, 1.0, a)[..., None])
+    return q, (a / 127.0).float().double()
+
+
+def ref_linear(x, w, b):
+    (qx, sx), (qw, sw) = ref_codes(x), ref_codes(w)
+    part = (qx @ qw.t()) * sx[..., None] * sw
+    return part + (0 if b is None else b.double().cpu()), part
+
+
+def check(x, w, b, y):
+    want, part = ref_linear(x, w, b)
+    assert y.dtype == x.dtype and y.shape == want.shape
+    tol = 6 * U * (part.abs() + want.abs()) + (0 if x.dtype == torch.float32 else torch.finfo(x.dtype).eps / 2) * want.abs()
+    if x.dtype == torch.float16:
+        tol = tol + 2.0 ** -25                 # half a step among its subnormals
+    off = (y.double().cpu() - want).abs()
+    assert bool((off <= tol).all()), (tuple(x.shape), tuple(w.shape), x.dtype, float((off - tol).max()))
+
+
+def data(m, k, n, dtype, bias, seed=0):
+    gen = torch.Generator("cuda").manual_seed(seed + 7 * m + 11 * k + 13 * n)
+    x = (torch.randn(m, k, device="cuda", generator=gen) * torch.exp(torch.randn(m, 1, device="cuda", generator=gen))).to(dtype)
+    w = torch.randn(n, k, device="cuda", generator=gen) * 0.03
+    return x, w, 0.1 * torch.randn(n, device="cuda", generator=gen) if bias else None
+
+
+@pytest.mark.parametrize("k", [1, 7, 128, 129, 333, 1000, 2048, 2049, 5000, 16384, 16385])
+@pytest.mark.parametrize("dtype", list(DT))
+def test_codes_and_scales(k, dtype):
+    from mmearth_train_amd.int8 import quantize_weight
+    for rows in (1, 5, 67):
+        x, _, _ = data(rows, k, 1, DT[dtype], False, 1)
+        if rows > 2:
+            x[1] = 0.0
+            x[2] *= 1e-3 if dtype == "fp16" else 1e-36
+            x[3, ::2] = x[3].abs().amax() / 2         # 63.5: exact ties, to even
+        w = quantize_weight(x)
+        q, s = ref_codes(x)
+        assert torch.equal(w.q[:, :k].cpu().double(), q), (rows, k, dtype)
+        assert torch.equal(w.scale.cpu().double(), s)
+        assert not w.q[:, k:].any()
+
+
+SHAPES = [(1, 1, 1), (1, 16, 16), (1, 1024, 4096), (1, 11264, 40), (2, 77, 1000), (3, 2816, 1000), (8, 2816, 1000), (15, 640, 129), (16, 640, 128), (17, 129, 640),
+          (33, 1000, 257), (49, 2816, 1408), (64, 320, 1280), (65, 320, 1280), (100, 43, 1009), (127, 160, 640), (128, 640, 160), (129, 5000, 255),
+          (255, 128, 512), (256, 512, 256), (257, 513, 259), (300, 1, 300), (1003, 333, 77), (511, 1024, 1025), (2000, 384, 96), (4099, 80, 320)]
+
+
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("m,k,n", SHAPES)
+def test_linear(m, k, n, dtype):
+    from mmearth_train_amd.int8 import linear_int8, quantize_weight
+    for bias in (True, False):
+        x, w, b = data(m, k, n, DT[dtype], bias)
+        check(x, w, b, linear_int8(x, quantize_weight(w, b)))
+
+
+@pytest.mark.parametrize("m", [1, 2, 5, 16, 17, 40, 64, 65, 200, 1030])
+def test_row_counts_around_every_variant(m):
+    from mmearth_train_amd.int8 import linear_int8, quantize_weight
+    for k, n in ((640, 1000), (2816, 704), (130, 4096)):
+        x, w, b = data(m, k, n, torch.bfloat16, True, 3)
+        check(x, w, b, linear_int8(x, quantize_weight(w, b)))
+
+
+def test_leading_dimensions_strides_and_offsets():
+    from mmearth_train_amd.int8 import linear_int8, quantize_weight
+    gen = torch.Generator("cuda").manual_seed(5)
+    w = torch.randn(90, 70, device="cuda", generator=gen)
+    p = quantize_weight(w)
+    for dtype in DT.values():
+        room = torch.randn(6, 5, 4, 200, device="cuda", generator=gen).to(dtype)
+        for x in (room[..., :70], room[..., 3:73], room[2, 1, 0, 1:71], room[0, 0, :, 5:75], room.permute(3, 0, 1, 2)[:4, :, :, 0].new_tensor(0).expand(3, 70),
+                  room[0, 0, :, :70].t().contiguous().t(), room[:0, ..., :70], room[:, :, :, :70].transpose(0, 2)):
+            y = linear_int8(x, p)
+            assert y.shape == x.shape[:-1] + (90,)
+            if x.numel():
+                check(x.reshape(-1, 70), w, None, y.reshape(-1, 90))
+    # a weight that is a view of another order
+    q = quantize_weight(w.t().contiguous().t())
+    assert torch.equal(q.q, p.q) and torch.equal(q.scale, p.scale)
+
+
+@pytest.mark.parametrize("m", [3, 70, 600])
+def test_bad_rows_stay_alone(m):
+    from mmearth_train_amd.int8 import linear_int8, quantize_weight
+    for dtype in DT.values():
+        x, w, b = data(m, 300, 130, dtype, True, 4)
+        p = quantize_weight(w, b)
+        x[0] = 0.0
+        clean = linear_int8(x, p)
+        assert torch.equal(clean[0].float(), b.to(dtype).float())
+        x[1, 299] = float("inf")
+        x[m - 1, 0] = float("nan")
+        y = linear_int8(x, p)
+        assert bool(torch.isnan(y[1]).all()) and bool(torch.isnan(y[m - 1]).all())
+        rest = [i for i in range(m) if i not in (1, m - 1)]
+        assert torch.equal(y[rest], clean[rest])
+
+
+def test_sums_of_the_largest_codes():
+    """Every product 127 * 127, the longest row whose sum fits 32 bits, both signs."""
+    from mmearth_train_amd.int8 import MAX_K, linear_int8, quantize_weight
+    for k in (MAX_K, MAX_K - 130):
+        for m in (1, 20, 300):
+            x, w = torch.ones(m, k, device="cuda", dtype=torch.bfloat16), torch.ones(3, k, device="cuda")
+            w[1] = -1.0
+            x[m - 1] = -2.0
+            check(x, w, None, linear_int8(x, quantize_weight(w)))
+
+
+def test_rows_past_31_bits():
+    """x of more than 2^31 elements: offsets of rows need 64 bits, in x, in the codes and in y."""
+    from mmearth_train_amd.int8 import linear_int8, quantize_weight
+    m, k, n = 2 ** 31 // 128 + 77, 128, 136
+    x = torch.zeros(m, k, device="cuda", dtype=torch.bfloat16)
+    tail = torch.randn(300, k, device="cuda", generator=torch.Generator("cuda").manual_seed(6)).to(torch.bfloat16)
+    x[-300:] = tail
+    w = torch.randn(n, k, device="cuda", generator=torch.Generator("cuda").manual_seed(7))
+    p = quantize_weight(w)
+    y = linear_int8(x, p)
+    check(tail, w, None, y[-300:])
+    assert not bool(y[:-300].any())
+
+
+def test_streams_and_graphs():
+    from mmearth_train_amd.int8 import linear_int8, quantize_weight
+    for m in (1, 40, 700):
+        x, w, b = data(m, 640, 512, torch.bfloat16, True, 8)
+        p = quantize_weight(w, b)
+        want = linear_int8(x, p)
+        s = torch.cuda.Stream()
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            y = linear_int8(x, p)
+        torch.cuda.current_stream().wait_stream(s)
+        assert torch.equal(y, want)
+        one, two = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()       # two graphs over one weight, replayed in turn
+        torch.cuda.synchronize()
+        with torch.cuda.graph(one):
+            y1 = linear_int8(x, p)
+        x2 = x.clone()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(two):
+            y2 = linear_int8(x2, p)
+        for k in range(3):
+            x.normal_(generator=torch.Generator("cuda").manual_seed(k))
+            x2.normal_(generator=torch.Generator("cuda").manual_seed(90 + k))
+            one.replay()
+            two.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(y1, linear_int8(x, p)) and torch.equal(y2, linear_int8(x2, p))
+
+
+def test_refusals_on_the_device():
+    from mmearth_train_amd.int8 import linear_int8, quantize_weight
+    w = torch.zeros(8, 16, device="cuda")
+    p = quantize_weight(w)
+    with pytest.raises(ValueError, match="end in 16"):
+        linear_int8(torch.zeros(2, 17, device="cuda"), p)
+    with pytest.raises(ValueError, match="end in 16"):
+        linear_int8(torch.zeros((), device="cuda"), p)
+    with pytest.raises(ValueError, match="fp32, bf16 or fp16"):
+        linear_int8(torch.zeros(2, 16, device="cuda", dtype=torch.float64), p)
+    with pytest.raises(ValueError, match="the input is on cpu"):
+        linear_int8(torch.zeros(2, 16), p)
+    x = torch.zeros(2, 16, device="cuda", requires_grad=True)
+    with pytest.raises(RuntimeError, match="no backward"):
+        linear_int8(x, p)
+    with torch.no_grad():
+        assert linear_int8(x, p).shape == (2, 8)
+    with pytest.raises(ValueError, match="bias"):
+        quantize_weight(w, torch.zeros(9, device="cuda"))
+
+
+def test_a_network_is_trained_with_8_bit_moments_and_served_in_int8(tmp_path):
+    """The dense network as a user has it: fine-tuned by the 8-bit AdamW, then quantised, saved, loaded and served."""
+    from mmearth_train_amd import convnextv2
+    from mmearth_train_amd.helpers import param_groups_weight_decay
+    from mmearth_train_amd.int8 import Int8Linear, quantize_model
+    from mmearth_train_amd.optim import AdamW
+    torch.manual_seed(0)
+    net = convnextv2.convnextv2_atto(num_classes=5).cuda()
+    opt = AdamW(param_groups_weight_decay(net, 0.05), lr=1e-3, betas=(0.9, 0.95), state_bits=8, max_norm=1.0)
+    x, t = torch.randn(6, 12, 56, 56, device="cuda"), torch.tensor([0, 1, 2, 3, 4, 0], device="cuda")
+    for _ in range(3):
+        loss = nn_loss(net(x), t)
+        loss.backward()
+        assert all(p.grad is not None and bool(torch.isfinite(p.grad).all()) for p in net.parameters())
+        opt.step()
+        opt.zero_grad()
+    assert opt.plan.steps.tolist() == [3] * len(opt.plan.params) and math.isfinite(float(opt.grad_norm))
+    with torch.no_grad():
+        # the same network with its weights and activations rounded as the definition rounds them
+        taken = {}
+        hooks = [mod.register_forward_hook(lambda mod, i, o, name=name: taken.__setitem__(name, (i[0], mod))) for name, mod in net.named_modules()
+                 if isinstance(mod, torch.nn.Linear)]
+        net(x)
+        for h in hooks:
+            h.remove()
+        assert len(taken) == 2 * 12 + 1
+        served = quantize_model(net)
+        mods = dict(served.named_modules())
+        assert sum(isinstance(v, Int8Linear) for v in mods.values()) == len(taken) and not any(isinstance(v, torch.nn.Linear) for v in mods.values())
+        for name, (i, linear) in taken.items():
+            check(i.reshape(-1, i.shape[-1]), linear.weight, linear.bias, mods[name](i).reshape(-1, linear.out_features))
+        y = served(x)
+        assert y.shape == (6, 5) and bool(torch.isfinite(y).all())
+        torch.save(served.state_dict(), tmp_path / "served.pth")
+        other = quantize_model(convnextv2.convnextv2_atto(num_classes=5).cuda())
+        other.load_state_dict(torch.load(tmp_path / "served.pth", map_location="cuda", weights_only=True))
+        # (F.layer_norm and the convolutions are the same calls on the same inputs)
+        assert torch.equal(other(x), y)
+        half = other.half()
+        lin = half.head
+        assert lin.scale.dtype == torch.float32 and lin.q.dtype == torch.int8
+        assert half(x.half()).dtype == torch.float16
+
+
+def nn_loss(y, t):
+    return torch.nn.functional.cross_entropy(y, t)
+
+
+def test_hub_serves_in_int8():
+    import hubconf
+    from mmearth_train_amd.int8 import Int8Linear
+    net = hubconf.MPMAE("convnextv2_atto", pretrained=False, num_classes=7, int8=True)
+    assert isinstance(net.head, Int8Linear) and isinstance(net.stages[0][0].pwconv1, Int8Linear) and net.head.q.is_cuda
+    with torch.no_grad():
+        assert net(torch.randn(1, 12, 56, 56, device="cuda")).shape == (1, 7)

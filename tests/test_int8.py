@@ -1,0 +1,67 @@
+"""Host side of the int8 linear layer: refusals, struct layout. No GPU."""
+import ctypes as C
+import os
+import subprocess
+
+import pytest
+import torch
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+
+
+@pytest.mark.parametrize("w,b,what", [
+    (torch.zeros(4), None, "matrix"), (torch.zeros(0, 4), None, "matrix"), (torch.zeros(4, 0), None, "matrix"),
+    (torch.zeros(4, 4, dtype=torch.float64), None, "fp32, bf16 or fp16"), (torch.zeros(4, 4, dtype=torch.int8), None, "fp32, bf16 or fp16"),
+    (torch.zeros(1, 131072), None, "at most 131071"), (torch.zeros(4, 4), torch.zeros(5), "bias"), (torch.zeros(4, 4), None, "GPU only"),
+])
+def test_refused_weights(w, b, what):
+    from mmearth_train_amd.int8 import quantize_weight
+    with pytest.raises(ValueError, match=what):
+        quantize_weight(w, b)
+
+
+def test_library_refuses_bad_arguments():
+    """An error instead of a launch: no GPU is touched."""
+    from mmearth_train_amd import _lib
+    lib = _lib.load()
+    room = C.create_string_buffer(4096)
+    at = (C.addressof(room) + 15) & ~15
+    for bad in ((3, at, 8, 1, 8, at, 128, at), (0, None, 8, 1, 8, at, 128, at), (0, at, 8, 0, 8, at, 128, at), (0, at, 8, 1, 0, at, 128, at), (0, at, -1, 1, 8, at, 128, at),
+                (0, at, 8, 1, 8, at, 64, at), (0, at, 8, 1, 129, at, 128, at), (0, at, 8, 1, 8, at + 4, 128, at), (0, at, 8, 1, 131072, at, 131072, at)):
+        assert lib.mpmae_quant_i8(*bad, None) != 0, bad
+    full = dict(x=at, q=at, sx=at, w=at, sw=at, bias=None, y=at, ldx=8, ldy=4, M=1, N=4, K=8, ldq=128, ldw=128)
+    for bad in (dict(N=0), dict(w=None), dict(sw=None), dict(y=None), dict(ldy=3), dict(ldw=256), dict(w=at + 8), dict(M=-1), dict(ldq=100)):
+        assert lib.mpmae_linear_i8(0, C.byref(_lib.I8Args(**{**full, **bad})), None) != 0, bad
+    assert lib.mpmae_linear_i8(5, C.byref(_lib.I8Args(**full)), None) != 0
+    assert lib.mpmae_linear_i8(0, None, None) != 0
+
+
+def test_struct_matches_the_header(tmp_path):
+    from mmearth_train_amd import _lib
+    src = tmp_path / "s.c"
+    src.write_text('#include <stdio.h>\n#include "mpmae_hip.h"\nint main(void) { printf("%zu %zu %zu\\n", sizeof(MpmaeI8Args), offsetof(MpmaeI8Args, ldx), '
+                   "offsetof(MpmaeI8Args, ldw)); return 0; }\n")
+    subprocess.run(["gcc", "-I", os.path.join(ROOT, "include"), str(src), "-o", str(tmp_path / "s")], check=True)
+    got = [int(x) for x in subprocess.run([str(tmp_path / "s")], check=True, capture_output=True, text=True).stdout.split()]
+    assert got == [C.sizeof(_lib.I8Args), _lib.I8Args.ldx.offset, _lib.I8Args.ldw.offset]
+
+
+def test_module_tree_and_moves():
+    from mmearth_train_amd.int8 import Int8Linear
+    m = Int8Linear(100, 7)
+    assert set(m.state_dict()) == {"q", "scale", "bias"} and m.q.shape == (7, 128)
+    assert set(Int8Linear(100, 7, bias=False).state_dict()) == {"q", "scale"}
+    h = m.half()
+    assert h.scale.dtype == torch.float32 and h.bias.dtype == torch.float32 and h.q.dtype == torch.int8
+    assert m.to("meta").q.device.type == "meta"
+
+
+def test_rows_of_any_input():
+    from mmearth_train_amd.int8 import _rows
+    x = torch.arange(240.0).reshape(4, 6, 10)
+    for v, ld in ((x, 10), (x[0], 10), (x[0, :, :7], 10), (x[0, 0], 10), (x[:, 0], 60)):
+        r, m, d = _rows(v, v.shape[-1])
+        assert r.shape == (m, v.shape[-1]) and (d == ld or m == 1) and (v.shape[-1] == 1 or r.stride(1) == 1)
+        assert torch.equal(r, v.reshape(-1, v.shape[-1]))
+    r, m, d = _rows(x[0].t(), 6)
+    assert r.stride(1) == 1 and torch.equal(r, x[0].t())
