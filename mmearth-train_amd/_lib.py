@@ -162,7 +162,7 @@ class AdamwArgs(C.Structure):
 
 class I8Args(C.Structure):
     _fields_ = [("x", c_void_p), ("q", c_void_p), ("sx", c_void_p), ("w", c_void_p), ("sw", c_void_p), ("bias", c_void_p), ("y", c_void_p),
-                ("ldx", C.c_longlong), ("ldy", C.c_longlong),
+                ("part", c_void_p), ("ldx", C.c_longlong), ("ldy", C.c_longlong),
                 ("M", c_int), ("N", c_int), ("K", c_int), ("ldq", c_int), ("ldw", c_int), ("pad_", c_int)]
 
 
@@ -277,6 +277,7 @@ SYMBOLS = {
 OTHER_SYMBOLS = {
     "mpmae_program_create": ([], c_void_p),
     "mpmae_program_destroy": ([c_void_p], None),
+    "mpmae_linear_i8_part_bytes": ([c_int, c_int, c_int], C.c_longlong),
 }
 
 _lib = None

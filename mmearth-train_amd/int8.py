@@ -85,9 +85,11 @@ def linear_int8(x, w):
         return y
     x, m, ld = _rows(x, w.k)
     kp = w.q.shape[1]
-    ws = torch.empty(m * (kp + 4), dtype=torch.uint8, device=x.device)       # codes, then scales
+    part = _lib.load().mpmae_linear_i8_part_bytes(m, w.n, w.k)
+    at_part = -(-m * (kp + 4) // 16) * 16
+    ws = torch.empty(at_part + part, dtype=torch.uint8, device=x.device)       # codes, scales, partial sums
     at = ws.data_ptr()
-    args = _lib.I8Args(x.data_ptr(), at, at + m * kp, w.q.data_ptr(), w.scale.data_ptr(), None if w.bias is None else w.bias.data_ptr(), y.data_ptr(),
+    args = _lib.I8Args(x.data_ptr(), at, at + m * kp, w.q.data_ptr(), w.scale.data_ptr(), None if w.bias is None else w.bias.data_ptr(), y.data_ptr(), at + at_part,
                        ld, w.n, m, w.n, w.k, kp, kp, 0)
     if torch.cuda.current_device() == x.device.index:
         err = _lib.load().mpmae_linear_i8(dt, C.byref(args), _stream(x.device))

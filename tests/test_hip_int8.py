@@ -83,6 +83,23 @@ def test_row_counts_around_every_variant(m):
         check(x, w, b, linear_int8(x, quantize_weight(w, b)))
 
 
+@pytest.mark.parametrize("m,k,n", [
+    (1500, 300, 1300), (3000, 200, 2300), (3000, 1100, 2300), (20000, 130, 2600), (4100, 2050, 4100), (4100, 2050, 4000), (5600, 2050, 5500), (8192, 2048, 2048),
+    (49, 11264, 2816), (20, 4097, 130), (100, 9000, 333), (33, 5000, 61), (9, 16384, 8300), (5, 3064, 515), (8, 2050, 70), (7, 1032, 333), (3, 6136, 100)])
+def test_every_variant_of_the_product(m, k, n):
+    """Sizes on both sides of every rule that chooses a kernel, against the products of the codes in 64 bits (exact: below 2^53) on the GPU."""
+    from mmearth_train_amd.int8 import linear_int8, quantize_weight
+    x, w, b = data(m, k, n, torch.bfloat16, True, 9)
+    p, q = quantize_weight(w, b), quantize_weight(x)
+    qx, _ = ref_codes(x[:50])
+    assert torch.equal(q.q[:50, :k].cpu().double(), qx)
+    part = (q.q[:, :k].double() @ p.q[:, :k].double().t().contiguous()) * q.scale.double()[:, None] * p.scale.double()
+    want = part + b.double()
+    y = linear_int8(x, p)
+    tol = 6 * U * (part.abs() + want.abs()) + torch.finfo(torch.bfloat16).eps / 2 * want.abs()
+    assert bool(((y.double() - want).abs() <= tol).all())
+
+
 def test_leading_dimensions_strides_and_offsets():
     from mmearth_train_amd.int8 import linear_int8, quantize_weight
     gen = torch.Generator("cuda").manual_seed(5)
