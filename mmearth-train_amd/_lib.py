@@ -326,3 +326,22 @@ def nondefault_options():
 def check(err: int, what: str):
     if err != 0:
         raise HipLibraryError(f"{what} failed with hipError {err}")
+
+
+_host = None
+
+
+def host_tensors():
+    """The native host side of the many-tensor and int8 operators (csrc/host_tensors.cpp); raises HipLibraryError if it is not built."""
+    global _host
+    if _host is None:
+        import importlib.machinery
+        import importlib.util
+        load()
+        path = os.path.join(_HERE, "_host_tensors.so")
+        if not os.path.isfile(path):
+            raise HipLibraryError(f"{path} not found: build it with `python -c 'import __graft_entry__ as g; g.build()'`")
+        loader = importlib.machinery.ExtensionFileLoader("_host_tensors", path)
+        _host = importlib.util.module_from_spec(importlib.util.spec_from_loader("_host_tensors", loader))
+        loader.exec_module(_host)
+    return _host

@@ -3,10 +3,14 @@
 // A Python loop over `p.data_ptr(), p.grad, p.grad.data_ptr()` and the checks costs ~0.6 us per tensor; for the 144 tensors of the smallest
 // network that is several times the kernel's own run time.
 #include <ATen/core/Tensor.h>
+#include <ATen/core/grad_mode.h>
+#include <ATen/ops/empty.h>
+#include <c10/core/DeviceGuard.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <Python.h>
 #include <cstdint>
 #include <exception>
+#include "../../include/mpmae_hip.h"
 
 namespace {
 
@@ -82,7 +86,57 @@ PyObject* gather(PyObject*, PyObject* args) {
   }
 }
 
-PyMethodDef methods[] = {{"gather", gather, METH_VARARGS, "addresses of parameters and gradients"}, {nullptr, nullptr, 0, nullptr}};
+// linear_i8(x, q, scale, bias or None, k, stream, address of mpmae_linear_i8, of mpmae_linear_i8_part_bytes) -> y. The checks, the output, the workspace and the call
+// of one int8 linear layer: in Python they take 11 us, longer than the kernel for a single row.
+PyObject* linear_i8(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  if (nargs != 8 || !THPVariable_Check(args[0]) || !THPVariable_Check(args[1]) || !THPVariable_Check(args[2]) || (args[3] != Py_None && !THPVariable_Check(args[3])))
+    return PyErr_Format(PyExc_TypeError, "linear_i8(x, q, scale, bias, k, stream, entry, part_bytes)");
+  const long long k = PyLong_AsLongLong(args[4]);
+  void* const stream = PyLong_AsVoidPtr(args[5]);
+  const auto entry = reinterpret_cast<int (*)(int, const MpmaeI8Args*, mpmae_stream_t)>(PyLong_AsVoidPtr(args[6]));
+  const auto part_bytes = reinterpret_cast<long long (*)(int, int, int)>(PyLong_AsVoidPtr(args[7]));
+  if (PyErr_Occurred()) return nullptr;
+  try {
+    at::Tensor x = THPVariable_Unpack(args[0]);
+    const at::Tensor &q = THPVariable_Unpack(args[1]), &scale = THPVariable_Unpack(args[2]);
+    if (x.requires_grad() && at::GradMode::is_enabled()) return PyErr_Format(PyExc_RuntimeError, "linear_int8 has no backward pass: call it under torch.no_grad()");
+    const int dt = code_of(x.scalar_type());
+    if (dt < 0 || x.layout() != at::kStrided) return PyErr_Format(PyExc_ValueError, "inputs are dense fp32, bf16 or fp16 tensors, not %s", c10::toString(x.scalar_type()));
+    if (x.dim() < 1 || x.size(-1) != k) return PyErr_Format(PyExc_ValueError, "inputs end in %lld elements, the weight's", k);
+    if (x.device() != q.device() || !x.device().is_cuda())
+      return PyErr_Format(PyExc_ValueError, "the input is on %s, the weight on %s", x.device().str().c_str(), q.device().str().c_str());
+    const int64_t n = q.size(0), kp = q.size(1);
+    at::DimVector shape(x.sizes().begin(), x.sizes().end());
+    shape.back() = n;
+    c10::OptionalDeviceGuard guard(x.device());
+    at::Tensor y = at::empty(shape, x.options().requires_grad(false));
+    if (y.numel()) {
+      if (x.dim() != 2 || (x.stride(1) != 1 && k > 1)) {
+        x = x.reshape({-1, k});
+        if (x.stride(1) != 1 && k > 1) x = x.contiguous();
+      }
+      const int64_t m = x.size(0);
+      if (m > INT32_MAX || n > INT32_MAX) return PyErr_Format(PyExc_ValueError, "more than 2^31 - 1 rows");
+      const int64_t codes = m * (kp + 4), part_at = (codes + 15) / 16 * 16;
+      const at::Tensor ws = at::empty({part_at + part_bytes((int)m, (int)n, (int)k)}, x.options().dtype(at::kByte).requires_grad(false));
+      char* at = static_cast<char*>(ws.data_ptr());
+      MpmaeI8Args a{};
+      a.x = x.data_ptr(); a.q = reinterpret_cast<int8_t*>(at); a.sx = reinterpret_cast<float*>(at + m * kp);
+      a.w = static_cast<const int8_t*>(q.data_ptr()); a.sw = static_cast<const float*>(scale.data_ptr());
+      a.bias = args[3] == Py_None ? nullptr : static_cast<const float*>(THPVariable_Unpack(args[3]).data_ptr());
+      a.y = y.data_ptr(); a.part = reinterpret_cast<int*>(at + part_at);
+      a.ldx = x.stride(0); a.ldy = n; a.M = (int)m; a.N = (int)n; a.K = (int)k; a.ldq = (int)kp; a.ldw = (int)kp;
+      if (const int err = entry(dt, &a, stream)) return PyErr_Format(PyExc_RuntimeError, "linear_i8 failed with hipError %d", err);
+    }
+    return THPVariable_Wrap(std::move(y));
+  } catch (const std::exception& e) {
+    PyErr_SetString(PyExc_RuntimeError, e.what());
+    return nullptr;
+  }
+}
+
+PyMethodDef methods[] = {{"gather", gather, METH_VARARGS, "addresses of parameters and gradients"},
+                         {"linear_i8", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(linear_i8)), METH_FASTCALL, "int8 linear layer"}, {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host_tensors", nullptr, -1, methods};
 
 }  // namespace

@@ -33,6 +33,16 @@ def _stream(device):
     return torch.cuda.current_stream(device).cuda_stream
 
 
+_native = None          # (native call, address of mpmae_linear_i8, of mpmae_linear_i8_part_bytes), from the first call on
+
+
+def _load_native():
+    global _native
+    lib, host = _lib.load(), _lib.host_tensors()
+    _native = (host.linear_i8, *(C.cast(f, C.c_void_p).value for f in (lib.mpmae_linear_i8, lib.mpmae_linear_i8_part_bytes)))
+    return _native
+
+
 class Int8Weight:
     """A weight matrix [N, K] as int8 codes with one scale per row, laid out for `linear_int8`. Made by `quantize_weight`."""
 
@@ -71,33 +81,9 @@ def quantize_weight(weight, bias=None):
 
 def linear_int8(x, w):
     """y = x W^T + bias for x [..., K] fp32 / bf16 / fp16 on the weight's GPU; y has x's type. A row that holds NaN or infinity gives a row of NaN."""
-    if x.requires_grad and torch.is_grad_enabled():
-        raise RuntimeError("linear_int8 has no backward pass: call it under torch.no_grad()")
-    dt = _DTYPES.get(x.dtype)
-    if dt is None:
-        raise ValueError(f"inputs are fp32, bf16 or fp16, not {x.dtype}")
-    if x.dim() < 1 or x.shape[-1] != w.k:
-        raise ValueError(f"inputs end in {w.k} elements, the weight's: got {tuple(x.shape)}")
-    if x.device != w.device:
-        raise ValueError(f"the input is on {x.device}, the weight on {w.device}")
-    y = torch.empty(x.shape[:-1] + (w.n,), dtype=x.dtype, device=x.device)
-    if not y.numel():
-        return y
-    x, m, ld = _rows(x, w.k)
-    kp = w.q.shape[1]
-    part = _lib.load().mpmae_linear_i8_part_bytes(m, w.n, w.k)
-    at_part = -(-m * (kp + 4) // 16) * 16
-    ws = torch.empty(at_part + part, dtype=torch.uint8, device=x.device)       # codes, scales, partial sums
-    at = ws.data_ptr()
-    args = _lib.I8Args(x.data_ptr(), at, at + m * kp, w.q.data_ptr(), w.scale.data_ptr(), None if w.bias is None else w.bias.data_ptr(), y.data_ptr(), at + at_part,
-                       ld, w.n, m, w.n, w.k, kp, kp, 0)
-    if torch.cuda.current_device() == x.device.index:
-        err = _lib.load().mpmae_linear_i8(dt, C.byref(args), _stream(x.device))
-    else:
-        with torch.cuda.device(x.device):
-            err = _lib.load().mpmae_linear_i8(dt, C.byref(args), _stream(x.device))
-    _lib.check(err, "linear_i8")
-    return y
+    call, entry, part = _native or _load_native()
+    stream = torch._C._cuda_getCurrentRawStream(w.device.index) if w.device.type == "cuda" else 0
+    return call(x, w.q, w.scale, w.bias, w.k, stream, entry, part)          # checks, output, workspace and launch: csrc/host_tensors.cpp
 
 
 class Int8Linear(nn.Module):
@@ -106,7 +92,7 @@ class Int8Linear(nn.Module):
 
     def __init__(self, in_features, out_features, bias=True, device=None):
         super().__init__()
-        self.in_features, self.out_features = in_features, out_features
+        self.in_features, self.out_features, self._weight = in_features, out_features, None
         kp = -(-in_features // _lib.I8_KPAD) * _lib.I8_KPAD
         self.register_buffer("q", torch.zeros(out_features, kp, dtype=torch.int8, device=device))
         self.register_buffer("scale", torch.zeros(out_features, dtype=torch.float32, device=device))
@@ -127,7 +113,10 @@ class Int8Linear(nn.Module):
         return self
 
     def forward(self, x):
-        return linear_int8(x, Int8Weight(self.q, self.scale, self.bias, self.in_features))
+        w = self._weight
+        if w is None or w.q is not self.q or w.scale is not self.scale or w.bias is not self.bias:
+            w = self._weight = Int8Weight(self.q, self.scale, self.bias, self.in_features)
+        return linear_int8(x, w)
 
     def extra_repr(self):
         return f"in_features={self.in_features}, out_features={self.out_features}, bias={self.bias is not None}"

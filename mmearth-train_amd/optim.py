@@ -8,9 +8,6 @@ the global gradient norm in the same call. The fused pretraining step has its ow
 The update is torch.optim.AdamW's (main_pretrain.py:312-320); `state_dict()` has its layout, so checkpoints go both ways. There is no CPU form.
 """
 import ctypes as C
-import importlib.machinery
-import importlib.util
-import os
 
 import numpy as np
 import torch
@@ -21,21 +18,6 @@ BLOCK = 256          # elements that share a scale of the 8-bit moments; every t
 CHUNK = 4096         # elements per workgroup (ADAMW_CHUNK of csrc/optim.cuh)
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _TABLE = np.dtype([("n", "<i8"), ("off", "<i8"), ("group", "<i4"), ("dt", "<i4")])      # MpmaeAdamwTensor
-_host = None
-
-
-def _host_tensors():
-    """The native reader of tensor addresses (csrc/host_tensors.cpp); raises if it is not built."""
-    global _host
-    if _host is None:
-        path = os.path.join(os.path.dirname(os.path.abspath(__file__)), "_host_tensors.so")
-        if not os.path.isfile(path):
-            raise _lib.HipLibraryError(f"{path} not found: build it with `python -c 'import __graft_entry__ as g; g.build()'`")
-        loader = importlib.machinery.ExtensionFileLoader("_host_tensors", path)
-        _host = importlib.util.module_from_spec(importlib.util.spec_from_loader("_host_tensors", loader))
-        loader.exec_module(_host)
-    return _host
-
 
 def moment_layout(numels):
     """Offsets of the tensors in the flat moment buffers (each starts a block of its own) and the buffers' length."""
@@ -199,8 +181,7 @@ class AdamW(torch.optim.Optimizer):
     def _build(self):
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("run one eager step before capturing one: the state is made on the first")
-        _lib.load()
-        _host_tensors()
+        _lib.host_tensors()
         params = [p for g in self.param_groups for p in g["params"]]
         groups_of = [i for i, g in enumerate(self.param_groups) for _ in g["params"]]
         self._check_apart()
@@ -255,7 +236,7 @@ class AdamW(torch.optim.Optimizer):
             with torch.enable_grad():
                 loss = closure()
         plan = self.plan
-        grads, other = _host_tensors().gather(plan.params, plan.table_at, plan.device.index, plan.ptrs_at)
+        grads, other = _lib.host_tensors().gather(plan.params, plan.table_at, plan.device.index, plan.ptrs_at)
         if not grads:
             plan.norm_skip.zero_()
             return loss

@@ -248,7 +248,13 @@ def test_a_network_is_trained_with_8_bit_moments_and_served_in_int8(tmp_path):
         other.load_state_dict(torch.load(tmp_path / "served.pth", map_location="cuda", weights_only=True))
         # (F.layer_norm and the convolutions are the same calls on the same inputs)
         assert torch.equal(other(x), y)
-        half = other.half()
+        import copy
+        twin = copy.deepcopy(other)              # its own buffers, read by its own calls
+        for buf in other.buffers():
+            if buf.dtype == torch.int8:
+                buf.zero_()
+        assert torch.equal(twin(x), y) and not torch.equal(other(x), y)
+        half = twin.half()
         lin = half.head
         assert lin.scale.dtype == torch.float32 and lin.q.dtype == torch.int8
         assert half(x.half()).dtype == torch.float16

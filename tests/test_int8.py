@@ -65,3 +65,14 @@ def test_rows_of_any_input():
         assert torch.equal(r, v.reshape(-1, v.shape[-1]))
     r, m, d = _rows(x[0].t(), 6)
     assert r.stride(1) == 1 and torch.equal(r, x[0].t())
+
+
+def test_a_cpu_input_is_refused_and_modules_copy():
+    import copy
+    import pickle
+    from mmearth_train_amd.int8 import Int8Linear
+    m = Int8Linear(100, 7)
+    with pytest.raises(ValueError, match="is on cpu"):
+        m(torch.zeros(2, 100))
+    for other in (copy.deepcopy(m), pickle.loads(pickle.dumps(m))):
+        assert other.q.data_ptr() != m.q.data_ptr() and (other._weight is None or other._weight.q is other.q)

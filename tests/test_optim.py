@@ -111,8 +111,8 @@ def test_structs_match_the_header(tmp_path):
 
 def test_native_reader_refuses_what_it_cannot_address():
     """csrc/host_tensors.cpp raises instead of handing an address on: everything here is on the CPU, so nothing gets as far as an address."""
-    from mmearth_train_amd import optim
-    host = optim._host_tensors()
+    from mmearth_train_amd import _lib, optim
+    host = _lib.host_tensors()
     table, out = np.zeros(1, optim._TABLE), np.zeros(2, np.uint64)
     with pytest.raises(ValueError, match="device"):
         host.gather([torch.nn.Parameter(torch.zeros(3))], table.ctypes.data, 0, out.ctypes.data)
