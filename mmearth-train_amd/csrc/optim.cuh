@@ -79,38 +79,45 @@ template <> struct AdamwIo<_Float16> {
     *reinterpret_cast<h8*>(p) = a;
   }
 };
-// eight consecutive elements, `left` of them inside the tensor (the others read as 0 and are not written); vec: whole and 16-byte aligned
-template <typename T>
-__device__ __forceinline__ void adamw_ld8(const T* p, long long left, bool vec, float (&o)[8]) {
-  if (vec && left >= 8) { AdamwIo<T>::ld8v(p, o); return; }
+// Eight consecutive elements from i on; those at or past n read as 0 and are not written. FULL: all inside, 16-byte aligned. Loads are never behind a branch (one
+// is waited for where the branch joins): a ragged tensor's come from clamped addresses.
+template <typename T, bool FULL>
+__device__ __forceinline__ void adamw_ld8(const T* p, long long i, long long n, float (&o)[8]) {
+  if (FULL) { AdamwIo<T>::ld8v(p + i, o); return; }
 #pragma unroll
-  for (int i = 0; i < 8; ++i) o[i] = i < left ? AdamwIo<T>::ld(p + i) : 0.f;
-}
-template <typename T>
-__device__ __forceinline__ void adamw_st8(T* p, long long left, bool vec, const float (&o)[8]) {
-  if (vec && left >= 8) { AdamwIo<T>::st8v(p, o); return; }
+  for (int e = 0; e < 8; ++e) o[e] = AdamwIo<T>::ld(p + min(i + e, n - 1));
 #pragma unroll
-  for (int i = 0; i < 8; ++i) if (i < left) AdamwIo<T>::st(p + i, o[i]);
+  for (int e = 0; e < 8; ++e) o[e] = i + e < n ? o[e] : 0.f;
 }
+template <typename T, bool FULL>
+__device__ __forceinline__ void adamw_st8(T* p, long long i, long long n, const float (&o)[8]) {
+  if (FULL) { AdamwIo<T>::st8v(p + i, o); return; }
+#pragma unroll
+  for (int e = 0; e < 8; ++e) if (i + e < n) AdamwIo<T>::st(p + i + e, o[e]);
+}
+// a workgroup's chunk in the form that its tensor allows
+#define ADAMW_BY_TYPE(...)                                                                        \
+  if (t.dt == 0) { using T = float; __VA_ARGS__ }                                                 \
+  else if (t.dt == 1) { using T = bf16_t; __VA_ARGS__ }                                           \
+  else { using T = _Float16; __VA_ARGS__ }
 
 // ---------------------------------------------------------------------------------
 // Sum of squares of every gradient of the launch, in fp64 (a factor that went into 8-bit codes must not depend on the summation order): workgroup b
 // walks chunks first + b, first + b + gridDim, ...; one partial per workgroup, no atomics.
 // ---------------------------------------------------------------------------------
-template <typename T>
+template <typename T, bool FULL>
 __device__ __forceinline__ double adamw_sumsq_chunk(const T* g, long long n, long long base) {
-  const bool vec = (((uintptr_t)g) & 15) == 0;
-  double s = 0.0;
+  float x[2][8];
+  double s[4] = {0.0, 0.0, 0.0, 0.0};
 #pragma unroll
-  for (int it = 0; it < ADAMW_CHUNK / 2048; ++it) {
-    const long long i = base + it * 2048 + threadIdx.x * 8;
-    float x[8];
-    adamw_ld8(g + i, n - i, vec, x);
+  for (int it = 0; it < 2; ++it) adamw_ld8<T, FULL>(g, base + it * 2048 + threadIdx.x * 8, n, x[it]);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) s += (double)x[e] * (double)x[e];
-  }
-  return s;
+  for (int it = 0; it < 2; ++it)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) s[e & 3] += (double)x[it][e] * (double)x[it][e];
+  return (s[0] + s[1]) + (s[2] + s[3]);
 }
+static_assert(ADAMW_CHUNK == 2 * 2048, "two vectors of eight per thread");
 __global__ __launch_bounds__(256) void adamw_norm_kernel(AdamwPtrs ptrs, const AdamwTensor* __restrict__ tensors, const int2* __restrict__ chunks,
                                                          int nchunks, double* __restrict__ partials) {
   __shared__ double red[4];
@@ -121,9 +128,8 @@ __global__ __launch_bounds__(256) void adamw_norm_kernel(AdamwPtrs ptrs, const A
     const void* g = ptrs.at[ch.x - ptrs.first].g;
     if (!g) continue;
     const long long base = (long long)ch.y * ADAMW_CHUNK;
-    if (t.dt == 0) s += adamw_sumsq_chunk((const float*)g, t.n, base);
-    else if (t.dt == 1) s += adamw_sumsq_chunk((const bf16_t*)g, t.n, base);
-    else s += adamw_sumsq_chunk((const _Float16*)g, t.n, base);
+    const bool full = (((uintptr_t)g) & 15) == 0 && base + ADAMW_CHUNK <= t.n;
+    ADAMW_BY_TYPE(s += full ? adamw_sumsq_chunk<T, true>((const T*)g, t.n, base) : adamw_sumsq_chunk<T, false>((const T*)g, t.n, base);)
   }
   s = adamw_block_sum(s, red);
   if (threadIdx.x == 0) partials[blockIdx.x] = s;
@@ -168,18 +174,17 @@ __global__ __launch_bounds__(256) void adamw_hyper_kernel(AdamwGroups groups, co
 // ---------------------------------------------------------------------------------
 // fp32 moments
 // ---------------------------------------------------------------------------------
-template <typename T>
+template <typename T, bool FULL>
 __device__ __forceinline__ void adamw32_chunk(T* __restrict__ p, const T* __restrict__ g, float* __restrict__ m, float* __restrict__ v, long long n,
                                               long long base, const AdamwHyper& h) {
-  const bool vec = ((((uintptr_t)p) | ((uintptr_t)g)) & 15) == 0;
   const float b1 = (float)h.b1, c1 = (float)(h.c1 * h.coef), b2 = (float)h.b2, c2 = (float)(h.c2 * h.coef * h.coef);
 #pragma unroll
   for (int it = 0; it < ADAMW_CHUNK / 2048; ++it) {
     const long long i = base + it * 2048 + threadIdx.x * 8;
-    if (i >= n) return;
+    if (!FULL && i >= n) return;
     float pv[8], gv[8], mv[8], vv[8];
-    adamw_ld8(p + i, n - i, vec, pv);
-    adamw_ld8(g + i, n - i, vec, gv);
+    adamw_ld8<T, FULL>(p, i, n, pv);
+    adamw_ld8<T, FULL>(g, i, n, gv);
     ld8(m + i, mv);                       // the flat moment buffers are padded to whole blocks: zero behind the tensor, and zero they stay
     ld8(v + i, vv);
 #pragma unroll
@@ -188,7 +193,7 @@ __device__ __forceinline__ void adamw32_chunk(T* __restrict__ p, const T* __rest
       vv[e] = b2 * vv[e] + c2 * gv[e] * gv[e];
       pv[e] = pv[e] * h.decay - h.step * mv[e] / (sqrtf(vv[e]) * h.isbc2 + h.eps);
     }
-    adamw_st8(p + i, n - i, vec, pv);
+    adamw_st8<T, FULL>(p, i, n, pv);
     st8(m + i, mv);
     st8(v + i, vv);
   }
@@ -203,9 +208,9 @@ __global__ __launch_bounds__(256) void adamw32_kernel(AdamwPtrs ptrs, const Adam
   if (!g || (norm_skip && norm_skip[1] != 0.f)) return;
   const AdamwHyper h = hyper[ch.x];
   const long long base = (long long)ch.y * ADAMW_CHUNK;
-  if (t.dt == 0) adamw32_chunk((float*)p, (const float*)g, m + t.off, v + t.off, t.n, base, h);
-  else if (t.dt == 1) adamw32_chunk((bf16_t*)p, (const bf16_t*)g, m + t.off, v + t.off, t.n, base, h);
-  else adamw32_chunk((_Float16*)p, (const _Float16*)g, m + t.off, v + t.off, t.n, base, h);
+  const bool full = ((((uintptr_t)p) | ((uintptr_t)g)) & 15) == 0 && base + ADAMW_CHUNK <= t.n;
+  ADAMW_BY_TYPE(if (full) adamw32_chunk<T, true>((T*)p, (const T*)g, m + t.off, v + t.off, t.n, base, h);
+                else adamw32_chunk<T, false>((T*)p, (const T*)g, m + t.off, v + t.off, t.n, base, h);)
 }
 
 // ---------------------------------------------------------------------------------
@@ -215,82 +220,98 @@ __global__ __launch_bounds__(256) void adamw32_kernel(AdamwPtrs ptrs, const Adam
 // two fp32 numbers ((9 s + g) / 10), and the scale, and with it every code, must not depend on how a compiler groups the terms.
 // ---------------------------------------------------------------------------------
 __device__ __forceinline__ unsigned adamw_max32(unsigned x) {      // maximum over the 32 lanes of a half wave (bit patterns of non-negative floats)
-#pragma unroll
-  for (int d = 16; d; d >>= 1) x = max(x, (unsigned)__shfl_xor((int)x, d));
-  return x;
+  x = max(x, (unsigned)__builtin_amdgcn_mov_dpp((int)x, 0xb1, 0xf, 0xf, true));       // lanes 1 0 3 2
+  x = max(x, (unsigned)__builtin_amdgcn_mov_dpp((int)x, 0x4e, 0xf, 0xf, true));       // lanes 2 3 0 1
+  x = max(x, (unsigned)__builtin_amdgcn_mov_dpp((int)x, 0x141, 0xf, 0xf, true));      // 8 lanes mirrored
+  x = max(x, (unsigned)__builtin_amdgcn_mov_dpp((int)x, 0x140, 0xf, 0xf, true));      // 16 lanes mirrored
+  const auto y = __builtin_amdgcn_permlane16_swap(x, x, false, false);                // rows of 16: {0 0 2 2}, {1 1 3 3}
+  return max(y[0], y[1]);
 }
-__device__ __forceinline__ int adamw_code_m(double m, float s, bool direct) {       // |code| in 0..127
-  if (direct) return min((int)floor(127.0 * sqrt(fabs(m) / (double)s) + 0.5), 127);
-  const float t = 127.f * sqrtf(fabsf((float)m) / s);
-  const float f = floorf(t), r = t - f;
-  int k = (int)f + (r >= 0.5f ? 1 : 0);
-  if (fabsf(r - 0.5f) < 1e-3f) {
-    const double b = (double)f + 0.5;
-    k = (int)f + (fabs(m) * 16129.0 >= b * b * (double)s ? 1 : 0);
-  }
-  return min(k, 127);
+// The code next to a value. t: the code's fp32 estimate (off by less than 1e-3, so its whole part is at most one below); the border above that whole part is
+// compared in fp64. m: |m| >= (f + 1/2)^2 s / 127^2; the square is exact in fp32. v: v >= (f + 1/2)^4 s / 255^4.
+__device__ __forceinline__ float adamw_code_m(double m, float inv, double border) {       // |code|, 0..127
+  const float f = floorf(__builtin_amdgcn_sqrtf(fabsf((float)m) * inv)), b = f + 0.5f;
+  return fminf(f + (fabs(m) >= (double)(b * b) * border ? 1.f : 0.f), 127.f);
 }
-__device__ __forceinline__ int adamw_code_v(double v, float s, bool direct) {       // 0..255
-  int k;
-  if (direct) k = (int)floor(255.0 * sqrt(sqrt(v / (double)s)) + 0.5);
-  else {
-    const float t = 255.f * sqrtf(sqrtf((float)v / s));
-    const float f = floorf(t), r = t - f;
-    k = (int)f + (r >= 0.5f ? 1 : 0);
-    if (fabsf(r - 0.5f) < 1e-3f) {
-      const double b = (double)f + 0.5, b2 = b * b;
-      k = (int)f + (v * (65025.0 * 65025.0) >= b2 * b2 * (double)s ? 1 : 0);
-    }
-  }
-  return max(min(k, 255), v > 0.0 ? 1 : 0);
+__device__ __forceinline__ float adamw_code_v(double v, float inv, double border) {       // 0..255, at least 1 where v > 0
+  const float f = floorf(__builtin_amdgcn_sqrtf(__builtin_amdgcn_sqrtf((float)v * inv))), b = f + 0.5f;
+  const double b2 = (double)(b * b);
+  return fmaxf(fminf(f + (v >= b2 * b2 * border ? 1.f : 0.f), 255.f), v > 0.0 ? 1.f : 0.f);
 }
-template <typename T>
+template <typename T, bool FULL>
 __device__ __forceinline__ void adamw8_chunk(T* __restrict__ p, const T* __restrict__ g, uint8_t* __restrict__ mc, uint8_t* __restrict__ vc,
                                              float* __restrict__ ms, float* __restrict__ vs, long long n, long long base, const AdamwHyper& h) {
 #pragma clang fp contract(off)
-  const bool vec = ((((uintptr_t)p) | ((uintptr_t)g)) & 15) == 0;
 #pragma unroll 1
   for (int it = 0; it < ADAMW_CHUNK / 2048; ++it) {
     const long long blk = (base + it * 2048) / ADAMW_BLOCK + (threadIdx.x >> 5);
     const long long i = blk * ADAMW_BLOCK + (threadIdx.x & 31) * 8;
-    if (blk * ADAMW_BLOCK >= n) return;              // (uniform over the block's 32 lanes)
+    if (!FULL && blk * ADAMW_BLOCK >= n) return;     // (uniform over the block's 32 lanes)
     float pv[8], gv[8];
-    adamw_ld8(p + i, n - i, vec, pv);
-    adamw_ld8(g + i, n - i, vec, gv);
+    adamw_ld8<T, FULL>(p, i, n, pv);
+    adamw_ld8<T, FULL>(g, i, n, gv);
     uint2 mq = *reinterpret_cast<const uint2*>(mc + i), vq = *reinterpret_cast<const uint2*>(vc + i);
     const double am = (double)ms[blk] * (1.0 / 16129.0), av = (double)vs[blk] * (1.0 / (65025.0 * 65025.0));
+    mq.x ^= 0x80808080u; mq.y ^= 0x80808080u;        // signed bytes + 128: the byte conversions are unsigned
     double m[8], v[8];
     unsigned mx = 0, vx = 0;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const int km = (int)(int8_t)((e < 4 ? mq.x : mq.y) >> (8 * (e & 3)));
-      const unsigned kv = ((e < 4 ? vq.x : vq.y) >> (8 * (e & 3))) & 255u;
-      const double gd = (double)gv[e] * h.coef;
-      m[e] = h.b1 * ((double)(km * abs(km)) * am) + h.c1 * gd;
-      v[e] = h.b2 * ((double)((kv * kv) * (kv * kv)) * av) + h.c2 * gd * gd;
-      mx = max(mx, __float_as_uint(fabsf((float)m[e])));
+      const float km = (float)((e < 4 ? mq.x : mq.y) >> (8 * (e & 3)) & 255u) - 128.f, kv = (float)((e < 4 ? vq.x : vq.y) >> (8 * (e & 3)) & 255u);
+      const double gd = (double)gv[e] * h.coef, kv2 = (double)(kv * kv);
+      m[e] = h.b1 * ((double)(km * fabsf(km)) * am) + h.c1 * gd;
+      v[e] = h.b2 * (kv2 * kv2 * av) + h.c2 * gd * gd;
+      mx = max(mx, __float_as_uint((float)m[e]) & 0x7fffffffu);
       vx = max(vx, __float_as_uint((float)v[e]) & 0x7fffffffu);
-      pv[e] = pv[e] * h.decay - h.step * (float)m[e] / (sqrtf((float)v[e]) * h.isbc2 + h.eps);
     }
-    adamw_st8(p + i, n - i, vec, pv);
+    // one-instruction root and reciprocal (1 ulp each) unless eps is so small that a subnormal root would matter
+    if (h.eps >= 1e-12f) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        pv[e] = pv[e] * h.decay - h.step * (float)m[e] * __builtin_amdgcn_rcpf(__builtin_amdgcn_sqrtf((float)v[e]) * h.isbc2 + h.eps);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) pv[e] = pv[e] * h.decay - h.step * (float)m[e] / (sqrtf((float)v[e]) * h.isbc2 + h.eps);
+    }
+    adamw_st8<T, FULL>(p, i, n, pv);
     mx = adamw_max32(mx);
     vx = adamw_max32(vx);
-    // a block with a non-finite moment gets a NaN scale (its moments read back as NaN, as fp32 moments would stay); an empty one the scale 0
+    // a block with a non-finite moment gets a NaN scale (its moments read back as NaN, as fp32 moments would stay); an empty one the scale 0; codes 0 for both.
+    // Scales whose reciprocal is out of fp32's range go through fp64.
     const bool mbad = mx >= 0x7f800000u, vbad = vx >= 0x7f800000u;
-    const float sm = mbad ? NAN : __uint_as_float(mx), sv = vbad ? NAN : __uint_as_float(vx);
-    const bool mdir = sm < 1e-30f, vdir = sv < 1e-30f;
-    mq = make_uint2(0, 0); vq = make_uint2(0, 0);
+    const float sm = __uint_as_float(mx), sv = __uint_as_float(vx);
+    float km[8], kv[8];
+    if (!mbad && mx && sm < 1e-28f) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) km[e] = fminf((float)floor(127.0 * sqrt(fabs(m[e]) / (double)sm) + 0.5), 127.f);
+    } else {
+      const float inv = 16129.f / sm;
+      const double border = (double)sm * (1.0 / 16129.0);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) km[e] = adamw_code_m(m[e], inv, border);
+    }
+    if (!vbad && vx && sv < 1e-28f) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) kv[e] = fmaxf(fminf((float)floor(255.0 * sqrt(sqrt(v[e] / (double)sv)) + 0.5), 255.f), v[e] > 0.0 ? 1.f : 0.f);
+    } else {
+      const float inv = 65025.f * 65025.f / sv;
+      const double border = (double)sv * (1.0 / (65025.0 * 65025.0));
+#pragma unroll
+      for (int e = 0; e < 8; ++e) kv[e] = adamw_code_v(v[e], inv, border);
+    }
+    mq = vq = make_uint2(0, 0);
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      int km = 0, kv = 0;
-      if (!mbad && mx) { km = adamw_code_m(m[e], sm, mdir); km = m[e] < 0.0 ? -km : km; }
-      if (!vbad && vx) kv = adamw_code_v(v[e], sv, vdir);
-      if (e < 4) { mq.x |= ((unsigned)km & 255u) << (8 * e); vq.x |= (unsigned)kv << (8 * e); }
-      else { mq.y |= ((unsigned)km & 255u) << (8 * (e - 4)); vq.y |= (unsigned)kv << (8 * (e - 4)); }
+      const float biased = copysignf(km[e], (float)m[e]) + 128.f;
+      if (e < 4) { mq.x = __builtin_amdgcn_cvt_pk_u8_f32(biased, e, mq.x); vq.x = __builtin_amdgcn_cvt_pk_u8_f32(kv[e], e, vq.x); }
+      else { mq.y = __builtin_amdgcn_cvt_pk_u8_f32(biased, e - 4, mq.y); vq.y = __builtin_amdgcn_cvt_pk_u8_f32(kv[e], e - 4, vq.y); }
     }
+    const bool mlive = !mbad && mx, vlive = !vbad && vx;
+    mq.x = mlive ? mq.x ^ 0x80808080u : 0; mq.y = mlive ? mq.y ^ 0x80808080u : 0;
+    vq.x = vlive ? vq.x : 0; vq.y = vlive ? vq.y : 0;
     *reinterpret_cast<uint2*>(mc + i) = mq;
     *reinterpret_cast<uint2*>(vc + i) = vq;
-    if ((threadIdx.x & 31) == 0) { ms[blk] = sm; vs[blk] = sv; }
+    if ((threadIdx.x & 31) == 0) { ms[blk] = mbad ? NAN : sm; vs[blk] = vbad ? NAN : sv; }
   }
 }
 __global__ __launch_bounds__(256) void adamw8_kernel(AdamwPtrs ptrs, const AdamwTensor* __restrict__ tensors, const int2* __restrict__ chunks,
@@ -303,9 +324,9 @@ __global__ __launch_bounds__(256) void adamw8_kernel(AdamwPtrs ptrs, const Adamw
   if (!g || (norm_skip && norm_skip[1] != 0.f)) return;
   const AdamwHyper h = hyper[ch.x];
   const long long base = (long long)ch.y * ADAMW_CHUNK, sb = t.off / ADAMW_BLOCK;
-  if (t.dt == 0) adamw8_chunk((float*)p, (const float*)g, m + t.off, v + t.off, ms + sb, vs + sb, t.n, base, h);
-  else if (t.dt == 1) adamw8_chunk((bf16_t*)p, (const bf16_t*)g, m + t.off, v + t.off, ms + sb, vs + sb, t.n, base, h);
-  else adamw8_chunk((_Float16*)p, (const _Float16*)g, m + t.off, v + t.off, ms + sb, vs + sb, t.n, base, h);
+  const bool full = ((((uintptr_t)p) | ((uintptr_t)g)) & 15) == 0 && base + ADAMW_CHUNK <= t.n;
+  ADAMW_BY_TYPE(if (full) adamw8_chunk<T, true>((T*)p, (const T*)g, m + t.off, v + t.off, ms + sb, vs + sb, t.n, base, h);
+                else adamw8_chunk<T, false>((T*)p, (const T*)g, m + t.off, v + t.off, ms + sb, vs + sb, t.n, base, h);)
 }
 
 // the values the codes stand for, fp32: 2 + 1/32 bytes read and 8 written per element
