@@ -588,18 +588,19 @@ int mpmae_sumsq(const float* x, size_t n, float* out, mpmae_stream_t stream);
  *   m = b1 m + (1 - b1) coef g;  v = b2 v + (1 - b2) (coef g)^2;  p = p (1 - lr wd) - lr / (1 - b1^t) m / (sqrt(v) / sqrt(1 - b2^t) + eps)
  * A tensor without a gradient (NULL) is left alone and its step count stands; so does everything when the norm is not finite (norm_skip[1] = 1).
  * Steps are counted on the device, so a captured call replays as the next step.
- *   - ptrs (HOST): {parameter, gradient} address of every tensor, passed to the kernels by value; both in the same dense element order;
+ *   - grads (HOST): gradient address of every tensor, passed to the kernels by value; in the parameter's own dense element order;
  *   - groups (HOST): {lr, beta1, beta2, eps, weight_decay} of every parameter group;
  *   - tensors (device, MpmaeAdamwTensor[nt]), chunks (device, int pairs {tensor, index} of every 4096-element piece, by tensor), chunk_first (HOST, nt + 1):
  *     the static description; off is the tensor's first element in the moment buffers, a multiple of 256, so is every buffer's length;
  *   - bits = 32: m, v fp32. bits = 8: m int8 / v uint8 codes and one fp32 scale per 256 elements (ms, vs): m = ms k|k| / 127^2, v = vs (k / 255)^4.
  *     Padding behind a tensor must be zero and stays zero;
  *   - steps (device int[nt]), hyper (device, MPMAE_ADAMW_HYPER_BYTES * nt, scratch), partials (device double[npartials], scratch, used with max_norm;
- *     MPMAE_ADAMW_NORM_BLOCKS per started 200 tensors suffice), norm_skip (device float[2]: the norm before the clip, 1 if the step was skipped). */
+ *     MPMAE_ADAMW_NORM_BLOCKS per started 480 tensors suffice), norm_skip (device float[2]: the norm before the clip, 1 if the step was skipped). */
 #define MPMAE_ADAMW_HYPER_BYTES 56
-#define MPMAE_ADAMW_NORM_BLOCKS 1024
+#define MPMAE_ADAMW_NORM_BLOCKS 2048
 typedef struct MpmaeAdamwTensor {
   long long n, off;
+  void* p;
   int group, dt;            /* dt: 0 fp32, 1 bf16, 2 fp16 */
 } MpmaeAdamwTensor;
 typedef struct MpmaeAdamwArgs {
@@ -609,7 +610,7 @@ typedef struct MpmaeAdamwArgs {
   double max_norm;
   int nt, npartials, bits, pad_;
 } MpmaeAdamwArgs;
-int mpmae_adamw_multi(const MpmaeAdamwArgs* args, const void* const* ptrs, const double* groups, int ngroups, mpmae_stream_t stream);
+int mpmae_adamw_multi(const MpmaeAdamwArgs* args, const void* const* grads, const double* groups, int ngroups, mpmae_stream_t stream);
 /* fp32 values of n (a multiple of 256) 8-bit moments */
 int mpmae_adamw_values(const uint8_t* m_codes, const uint8_t* v_codes, const float* ms, const float* vs, float* m, float* v, long long n,
                        mpmae_stream_t stream);

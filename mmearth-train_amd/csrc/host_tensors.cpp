@@ -14,11 +14,6 @@
 
 namespace {
 
-struct Expected {            // the host copy of one record of the optimizer's tensor table
-  int64_t n, off;
-  int32_t group, dt;
-};
-
 int code_of(at::ScalarType t) { return t == at::kFloat ? 0 : t == at::kBFloat16 ? 1 : t == at::kHalf ? 2 : -1; }
 
 // same element order in memory: equal strides wherever a dimension has more than one element
@@ -29,19 +24,21 @@ bool same_order(const at::Tensor& a, const at::Tensor& b) {
   return true;
 }
 
-// gather(params, expected, device, out) -> (tensors with a gradient, None or [indices whose gradient lies in another element order])
-// expected: address of Expected[len(params)]; out: address of {parameter, gradient} pairs, gradient 0 where there is none.
+// gather(params, table, device, out) -> (tensors with a gradient, whether a parameter has moved, None or [indices whose gradient lies in another element order])
+// table: address of the host copy of MpmaeAdamwTensor[len(params)], whose parameter addresses are brought up to date; out: address of the gradients'
+// addresses, 0 where there is none.
 PyObject* gather(PyObject*, PyObject* args) {
   PyObject* list;
   unsigned long long expected_at, out_at;
   int device;
   if (!PyArg_ParseTuple(args, "O!KiK", &PyList_Type, &list, &expected_at, &device, &out_at)) return nullptr;
-  const Expected* want = reinterpret_cast<const Expected*>(expected_at);
+  MpmaeAdamwTensor* want = reinterpret_cast<MpmaeAdamwTensor*>(expected_at);
   uint64_t* out = reinterpret_cast<uint64_t*>(out_at);
   PyObject* other = nullptr;
   try {
     const Py_ssize_t count = PyList_GET_SIZE(list);
     Py_ssize_t grads = 0;
+    bool moved = false;
     for (Py_ssize_t i = 0; i < count; ++i) {
       PyObject* o = PyList_GET_ITEM(list, i);
       const char* wrong = nullptr;
@@ -53,15 +50,17 @@ PyObject* gather(PyObject*, PyObject* args) {
         else if (!p.is_non_overlapping_and_dense()) wrong = "is not dense in memory";
         else {
           const at::Tensor& g = p.grad();
-          out[2 * i] = reinterpret_cast<uint64_t>(p.data_ptr());
-          out[2 * i + 1] = 0;
+          void* const at = p.data_ptr();
+          moved |= want[i].p != at;
+          want[i].p = at;
+          out[i] = 0;
           if (g.defined()) {
             if (g.layout() != at::kStrided) wrong = "has a sparse gradient";
             else if (g.device() != p.device() || g.scalar_type() != p.scalar_type() || g.sizes() != p.sizes()) wrong = "has a gradient of another device, type or shape";
             else {
               ++grads;
               p.unsafeGetTensorImpl()->bump_version();      // the kernel writes it behind autograd's back: a stale saved tensor has to be noticed
-              if (same_order(p, g)) out[2 * i + 1] = reinterpret_cast<uint64_t>(g.data_ptr());
+              if (same_order(p, g)) out[i] = reinterpret_cast<uint64_t>(g.data_ptr());
               else {
                 if (!other && !(other = PyList_New(0))) return nullptr;
                 PyObject* k = PyLong_FromSsize_t(i);
@@ -78,7 +77,8 @@ PyObject* gather(PyObject*, PyObject* args) {
         return PyErr_Format(PyExc_ValueError, "parameter %zd %s", i, wrong);
       }
     }
-    return other ? Py_BuildValue("nN", grads, other) : Py_BuildValue("nO", grads, Py_None);
+    PyObject* const flag = moved ? Py_True : Py_False;
+    return other ? Py_BuildValue("nON", grads, flag, other) : Py_BuildValue("nOO", grads, flag, Py_None);
   } catch (const std::exception& e) {
     Py_XDECREF(other);
     PyErr_SetString(PyExc_RuntimeError, e.what());

@@ -13,26 +13,29 @@
 #pragma once
 #include "common.cuh"
 
-#define ADAMW_CHUNK 4096      // elements per workgroup of 256 threads
+#ifndef ADAMW_CHUNK
+#define ADAMW_CHUNK 4096
+#endif                        // elements per workgroup of 256 threads
 #define ADAMW_BLOCK 256       // elements per 8-bit block
-#define ADAMW_MAX_PTRS 200    // tensors per launch: their addresses travel in the kernel arguments (16 bytes each, 4 KB at most)
-#define ADAMW_MAX_GROUPS 64   // parameter groups per hyper launch (40 bytes each) and
+#define ADAMW_MAX_GRADS 480   // tensors per launch: the gradients' addresses travel in the kernel arguments (4 KB at most)
+#define ADAMW_MAX_GROUPS 48   // parameter groups per hyper launch (56 bytes each) and
 #define ADAMW_MAX_HAS 512     // tensors per hyper launch (one bit each: has a gradient)
 
 struct AdamwTensor {          // device table, one per parameter tensor (host mirror: MpmaeAdamwTensor)
   long long n, off;           // elements; first element in the flat moment buffers (a multiple of ADAMW_BLOCK)
+  void* p;
   int group, dt;              // parameter group; 0 fp32, 1 bf16, 2 fp16
 };
 struct AdamwHyper {           // device table, one per parameter tensor, written by adamw_hyper_kernel for this step
   double b1, c1, b2, c2, coef;      // c = 1 - b; coef: the clip factor
   float decay, step, isbc2, eps;
 };
-struct AdamwPtrs {
-  struct { void* p; const void* g; } at[ADAMW_MAX_PTRS];
+struct AdamwGrads {
+  const void* g[ADAMW_MAX_GRADS];
   int first;                  // index of the launch's first tensor
 };
 struct AdamwGroups {
-  struct { double lr, b1, b2, eps, wd; } at[ADAMW_MAX_GROUPS];
+  struct { double lr, b1, b2, eps, wd, ln_b1, ln_b2; } at[ADAMW_MAX_GROUPS];
   unsigned has[ADAMW_MAX_HAS / 32];
   int first, count, t0, t1;   // groups [first, first + count), tensors [t0, t1)
 };
@@ -107,29 +110,34 @@ __device__ __forceinline__ void adamw_st8(T* p, long long i, long long n, const 
 // ---------------------------------------------------------------------------------
 template <typename T, bool FULL>
 __device__ __forceinline__ double adamw_sumsq_chunk(const T* g, long long n, long long base) {
-  float x[2][8];
+  constexpr int IT = ADAMW_CHUNK / 2048;
+  float x[IT][8];
   double s[4] = {0.0, 0.0, 0.0, 0.0};
 #pragma unroll
-  for (int it = 0; it < 2; ++it) adamw_ld8<T, FULL>(g, base + it * 2048 + threadIdx.x * 8, n, x[it]);
+  for (int it = 0; it < IT; ++it) adamw_ld8<T, FULL>(g, base + it * 2048 + threadIdx.x * 8, n, x[it]);
 #pragma unroll
-  for (int it = 0; it < 2; ++it)
+  for (int it = 0; it < IT; ++it)
 #pragma unroll
     for (int e = 0; e < 8; ++e) s[e & 3] += (double)x[it][e] * (double)x[it][e];
   return (s[0] + s[1]) + (s[2] + s[3]);
 }
-static_assert(ADAMW_CHUNK == 2 * 2048, "two vectors of eight per thread");
-__global__ __launch_bounds__(256) void adamw_norm_kernel(AdamwPtrs ptrs, const AdamwTensor* __restrict__ tensors, const int2* __restrict__ chunks,
+__global__ __launch_bounds__(256) void adamw_norm_kernel(AdamwGrads grads, const AdamwTensor* __restrict__ tensors, const int2* __restrict__ chunks,
                                                          int nchunks, double* __restrict__ partials) {
   __shared__ double red[4];
   double s = 0.0;
+  // the next piece's description is read under the sum of the current one: three dependent reads would stand in front of every piece
+  int2 ch = chunks[blockIdx.x];
+  AdamwTensor t = tensors[ch.x];
   for (int c = blockIdx.x; c < nchunks; c += gridDim.x) {
-    const int2 ch = chunks[c];
-    const AdamwTensor t = tensors[ch.x];
-    const void* g = ptrs.at[ch.x - ptrs.first].g;
-    if (!g) continue;
+    const int2 ch_next = chunks[min(c + (int)gridDim.x, nchunks - 1)];
+    const void* g = grads.g[ch.x - grads.first];
     const long long base = (long long)ch.y * ADAMW_CHUNK;
-    const bool full = (((uintptr_t)g) & 15) == 0 && base + ADAMW_CHUNK <= t.n;
-    ADAMW_BY_TYPE(s += full ? adamw_sumsq_chunk<T, true>((const T*)g, t.n, base) : adamw_sumsq_chunk<T, false>((const T*)g, t.n, base);)
+    if (g) {
+      const bool full = (((uintptr_t)g) & 15) == 0 && base + ADAMW_CHUNK <= t.n;
+      ADAMW_BY_TYPE(s += full ? adamw_sumsq_chunk<T, true>((const T*)g, t.n, base) : adamw_sumsq_chunk<T, false>((const T*)g, t.n, base);)
+    }
+    ch = ch_next;
+    t = tensors[ch.x];
   }
   s = adamw_block_sum(s, red);
   if (threadIdx.x == 0) partials[blockIdx.x] = s;
@@ -139,22 +147,22 @@ __global__ __launch_bounds__(256) void adamw_norm_kernel(AdamwPtrs ptrs, const A
 // One workgroup: folds the norm's partials, decides on a skip (a non-finite norm leaves everything as it was, steps included), counts the steps of the
 // tensors that have a gradient and writes their records. 1 - b^t in fp64: at t = 1 it is a difference of near-equal numbers.
 // ---------------------------------------------------------------------------------
-__global__ __launch_bounds__(256) void adamw_hyper_kernel(AdamwGroups groups, const AdamwTensor* __restrict__ tensors,
+__global__ __launch_bounds__(512) void adamw_hyper_kernel(AdamwGroups groups, const AdamwTensor* __restrict__ tensors,
                                                           int* __restrict__ steps, AdamwHyper* __restrict__ hyper,
                                                           const double* __restrict__ partials, int npartials, double max_norm,
                                                           float* __restrict__ norm_skip) {
-  __shared__ double red[4];
+  __shared__ double red[8];
   float coef = 1.f;
   if (npartials > 0) {
     double s = 0.0;
-    for (int i = threadIdx.x; i < npartials; i += 256) s += partials[i];
+    for (int i = threadIdx.x; i < npartials; i += 512) s += partials[i];
     const double norm = sqrt(adamw_block_sum(s, red));
     const bool bad = !(norm < (double)INFINITY);
     if (threadIdx.x == 0) { norm_skip[0] = (float)norm; norm_skip[1] = bad ? 1.f : 0.f; }
     if (bad) return;
     coef = (float)fmin(1.0, max_norm / (norm + 1e-6));
   }
-  for (int i = groups.t0 + threadIdx.x; i < groups.t1; i += 256) {
+  for (int i = groups.t0 + threadIdx.x; i < groups.t1; i += 512) {
     const int g = tensors[i].group - groups.first;
     if (g < 0 || g >= groups.count || !(groups.has[(i - groups.t0) >> 5] >> ((i - groups.t0) & 31) & 1)) continue;
     const int t = steps[i] + 1;
@@ -164,8 +172,8 @@ __global__ __launch_bounds__(256) void adamw_hyper_kernel(AdamwGroups groups, co
     h.b1 = b1; h.b2 = b2;
     h.c1 = 1.0 - b1; h.c2 = 1.0 - b2; h.coef = (double)coef;
     h.decay = (float)(1.0 - lr * groups.at[g].wd);
-    h.step = (float)(lr / (1.0 - pow(b1, (double)t)));
-    h.isbc2 = (float)(1.0 / sqrt(1.0 - pow(b2, (double)t)));
+    h.step = (float)(lr / -expm1((double)t * groups.at[g].ln_b1));
+    h.isbc2 = (float)(1.0 / sqrt(-expm1((double)t * groups.at[g].ln_b2)));
     h.eps = (float)groups.at[g].eps;
     hyper[i] = h;
   }
@@ -198,13 +206,14 @@ __device__ __forceinline__ void adamw32_chunk(T* __restrict__ p, const T* __rest
     st8(v + i, vv);
   }
 }
-__global__ __launch_bounds__(256) void adamw32_kernel(AdamwPtrs ptrs, const AdamwTensor* __restrict__ tensors, const int2* __restrict__ chunks,
+__global__ __launch_bounds__(256) void adamw32_kernel(AdamwGrads grads, const AdamwTensor* __restrict__ tensors, const int2* __restrict__ chunks,
                                                       const AdamwHyper* __restrict__ hyper, float* __restrict__ m, float* __restrict__ v,
                                                       const float* __restrict__ norm_skip) {
-  const int2 ch = chunks[blockIdx.x];
+  // behind a norm the pieces are walked backwards: the gradients read last are the ones the memory-side cache still holds
+  const int2 ch = chunks[norm_skip ? gridDim.x - 1 - blockIdx.x : blockIdx.x];
   const AdamwTensor t = tensors[ch.x];
-  void* p = ptrs.at[ch.x - ptrs.first].p;
-  const void* g = ptrs.at[ch.x - ptrs.first].g;
+  void* p = t.p;
+  const void* g = grads.g[ch.x - grads.first];
   if (!g || (norm_skip && norm_skip[1] != 0.f)) return;
   const AdamwHyper h = hyper[ch.x];
   const long long base = (long long)ch.y * ADAMW_CHUNK;
@@ -314,13 +323,14 @@ __device__ __forceinline__ void adamw8_chunk(T* __restrict__ p, const T* __restr
     if ((threadIdx.x & 31) == 0) { ms[blk] = mbad ? NAN : sm; vs[blk] = vbad ? NAN : sv; }
   }
 }
-__global__ __launch_bounds__(256) void adamw8_kernel(AdamwPtrs ptrs, const AdamwTensor* __restrict__ tensors, const int2* __restrict__ chunks,
+__global__ __launch_bounds__(256) void adamw8_kernel(AdamwGrads grads, const AdamwTensor* __restrict__ tensors, const int2* __restrict__ chunks,
                                                      const AdamwHyper* __restrict__ hyper, uint8_t* __restrict__ m, uint8_t* __restrict__ v,
                                                      float* __restrict__ ms, float* __restrict__ vs, const float* __restrict__ norm_skip) {
-  const int2 ch = chunks[blockIdx.x];
+  // behind a norm the pieces are walked backwards: the gradients read last are the ones the memory-side cache still holds
+  const int2 ch = chunks[norm_skip ? gridDim.x - 1 - blockIdx.x : blockIdx.x];
   const AdamwTensor t = tensors[ch.x];
-  void* p = ptrs.at[ch.x - ptrs.first].p;
-  const void* g = ptrs.at[ch.x - ptrs.first].g;
+  void* p = t.p;
+  const void* g = grads.g[ch.x - grads.first];
   if (!g || (norm_skip && norm_skip[1] != 0.f)) return;
   const AdamwHyper h = hyper[ch.x];
   const long long base = (long long)ch.y * ADAMW_CHUNK, sb = t.off / ADAMW_BLOCK;

@@ -17,7 +17,7 @@ from . import _lib
 BLOCK = 256          # elements that share a scale of the 8-bit moments; every tensor starts at a multiple of it in the moment buffers
 CHUNK = 4096         # elements per workgroup (ADAMW_CHUNK of csrc/optim.cuh)
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
-_TABLE = np.dtype([("n", "<i8"), ("off", "<i8"), ("group", "<i4"), ("dt", "<i4")])      # MpmaeAdamwTensor
+_TABLE = np.dtype([("n", "<i8"), ("off", "<i8"), ("p", "<u8"), ("group", "<i4"), ("dt", "<i4")])      # MpmaeAdamwTensor
 
 def moment_layout(numels):
     """Offsets of the tensors in the flat moment buffers (each starts a block of its own) and the buffers' length."""
@@ -54,20 +54,20 @@ class _Plan:
         nt = len(params)
         self.table = np.zeros(nt, _TABLE)
         self.table["n"], self.table["off"], self.table["group"] = numels, self.offsets, groups_of
-        self.table["dt"] = [_DTYPES[p.dtype] for p in params]
+        self.table["dt"], self.table["p"] = [_DTYPES[p.dtype] for p in params], [p.data_ptr() for p in params]
         per = -(-self.table["n"] // CHUNK)
         self.chunk_first = np.zeros(nt + 1, np.int32)
         self.chunk_first[1:] = np.cumsum(per)
         chunks = np.empty((int(per.sum()), 2), np.int32)
         chunks[:, 0] = np.repeat(np.arange(nt), per)
         chunks[:, 1] = np.arange(len(chunks)) - np.repeat(self.chunk_first[:-1], per)
-        self.ptrs = np.zeros(2 * nt, np.uint64)
+        self.grads = np.zeros(nt, np.uint64)
         new = lambda n, dtype: torch.zeros(n, dtype=dtype, device=device)  # noqa: E731
         self.d_table = torch.from_numpy(self.table.view(np.uint8).copy()).to(device)
         self.d_chunks = torch.from_numpy(chunks).to(device)
         self.steps = new(nt, torch.int32)
         self.hyper = new(nt * _lib.ADAMW_HYPER_BYTES, torch.uint8)
-        npart = _lib.ADAMW_NORM_BLOCKS * (nt // 200 + 1)
+        npart = _lib.ADAMW_NORM_BLOCKS * (nt // 480 + 1)
         self.partials = new(npart if max_norm else 1, torch.float64)
         self.norm_skip = new(2, torch.float32)
         self.norm, self.skip = self.norm_skip[0], self.norm_skip[1]
@@ -80,8 +80,8 @@ class _Plan:
         self.args = _lib.AdamwArgs(tensors=at(self.d_table), chunks=at(self.d_chunks), chunk_first=self.chunk_first.ctypes.data, steps=at(self.steps),
                                    hyper=at(self.hyper), partials=at(self.partials), norm_skip=at(self.norm_skip), m=at(self.m), v=at(self.v),
                                    ms=at(self.ms), vs=at(self.vs), max_norm=float(max_norm or 0.0), nt=nt, npartials=npart, bits=bits)
-        self.ref = C.byref(self.args)
-        self.table_at, self.ptrs_at = self.table.ctypes.data, self.ptrs.ctypes.data
+        self.ref, self.stale = C.byref(self.args), False          # stale: parameters have moved and the device table does not know
+        self.table_at, self.grads_at = self.table.ctypes.data, self.grads.ctypes.data
         torch.cuda.current_stream(device).synchronize()      # the tables and zeroed moments are there for whatever stream steps first
 
     def values(self):
@@ -236,7 +236,14 @@ class AdamW(torch.optim.Optimizer):
             with torch.enable_grad():
                 loss = closure()
         plan = self.plan
-        grads, other = _lib.host_tensors().gather(plan.params, plan.table_at, plan.device.index, plan.ptrs_at)
+        grads, moved, other = _lib.host_tensors().gather(plan.params, plan.table_at, plan.device.index, plan.grads_at)
+        plan.stale |= moved
+        if plan.stale:                                 # (`p.data = ...`, `model.load_state_dict(assign=True)`)
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("a parameter has moved in memory: run one eager step before capturing one")
+            self._check_apart()
+            plan.d_table.copy_(torch.from_numpy(plan.table.view(np.uint8)))
+            plan.stale = False
         if not grads:
             plan.norm_skip.zero_()
             return loss
@@ -244,7 +251,7 @@ class AdamW(torch.optim.Optimizer):
         for i in other or ():
             p = plan.params[i]
             copies.append(torch.empty_like(p, memory_format=torch.preserve_format).copy_(p.grad))
-            plan.ptrs[2 * i + 1] = copies[-1].data_ptr()
+            plan.grads[i] = copies[-1].data_ptr()
         groups = []
         for g in self.param_groups:
             if isinstance(g["lr"], torch.Tensor):
@@ -260,7 +267,7 @@ class AdamW(torch.optim.Optimizer):
         return loss
 
     def _launch(self, plan, hyper):
-        return _lib.load().mpmae_adamw_multi(plan.ref, plan.ptrs_at, hyper, len(hyper) // 5, torch.cuda.current_stream(plan.device).cuda_stream)
+        return _lib.load().mpmae_adamw_multi(plan.ref, plan.grads_at, hyper, len(hyper) // 5, torch.cuda.current_stream(plan.device).cuda_stream)
 
     # ---- checkpoints: torch.optim.AdamW's layout -------------------------------------------------------------------------------------------
     def state_dict(self):

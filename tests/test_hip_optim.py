@@ -445,3 +445,35 @@ def test_main_pretrain_refuses_settings_that_would_do_nothing():
     for extra in (["--opt", "adamw"], ["--clip_grad", "1.0"], ["--fast_path", "False", "--clip_grad", "1.0"]):
         with pytest.raises(ValueError, match="--opt|--clip_grad"):
             main_pretrain.main(main_pretrain.get_args_parser().parse_args(base + extra))
+
+
+def test_parameters_that_move_in_memory():
+    """`p.data = other`: the step follows the parameter; a capture right after it is refused (the device table has to be written first)."""
+    from mmearth_train_amd.optim import AdamW
+    params, twin = params_of([300, 5000], DT[:2], 17), params_of([300, 5000], DT[:2], 17)
+    a, b = AdamW(params, state_bits=8), AdamW(twin, state_bits=8)
+    for k in range(3):
+        for ps in (params, twin):
+            grads_for(ps, 80 + k)
+        old = params[1].data
+        if k:
+            params[1].data = old.clone()
+        kept = old.clone()
+        a.step(), b.step()
+        assert all(torch.equal(p, q) for p, q in zip(params, twin))
+        assert k == 0 or torch.equal(old, kept)
+    params[0].data = params[0].data.clone()
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="moved"):
+        with torch.cuda.graph(graph):
+            a.step()
+    a.step(), b.step()
+    assert all(torch.equal(p, q) for p, q in zip(params, twin))
+    x = torch.zeros(600, device="cuda")
+    p, q = torch.nn.Parameter(x[:300]), torch.nn.Parameter(torch.zeros(300, device="cuda"))
+    c = AdamW([p, q])
+    p.grad, q.grad = torch.ones(300, device="cuda"), torch.ones(300, device="cuda")
+    c.step()
+    q.data = x[100:400]
+    with pytest.raises(ValueError, match="share memory"):
+        c.step()

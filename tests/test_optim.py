@@ -118,7 +118,7 @@ def test_native_reader_refuses_what_it_cannot_address():
         host.gather([torch.nn.Parameter(torch.zeros(3))], table.ctypes.data, 0, out.ctypes.data)
     with pytest.raises(ValueError, match="not a tensor"):
         host.gather([3], table.ctypes.data, 0, out.ctypes.data)
-    assert host.gather([], table.ctypes.data, 0, out.ctypes.data) == (0, None)
+    assert host.gather([], table.ctypes.data, 0, out.ctypes.data) == (0, False, None)
 
 
 @pytest.fixture(scope="module")
