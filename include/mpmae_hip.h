@@ -590,7 +590,7 @@ int mpmae_sumsq(const float* x, size_t n, float* out, mpmae_stream_t stream);
  * Steps are counted on the device, so a captured call replays as the next step.
  *   - grads (HOST): gradient address of every tensor, passed to the kernels by value; in the parameter's own dense element order;
  *   - groups (HOST): {lr, beta1, beta2, eps, weight_decay} of every parameter group;
- *   - tensors (device, MpmaeAdamwTensor[nt]), chunks (device, int pairs {tensor, index} of every 4096-element piece, by tensor), chunk_first (HOST, nt + 1):
+ *   - tensors (device, MpmaeAdamwTensor[nt]), chunks (device, int pairs {tensor, index} of every 2048-element piece, by tensor), chunk_first (HOST, nt + 1):
  *     the static description; off is the tensor's first element in the moment buffers, a multiple of 256, so is every buffer's length;
  *   - bits = 32: m, v fp32. bits = 8: m int8 / v uint8 codes and one fp32 scale per 256 elements (ms, vs): m = ms k|k| / 127^2, v = vs (k / 255)^4.
  *     Padding behind a tensor must be zero and stays zero;

@@ -13,9 +13,7 @@
 #pragma once
 #include "common.cuh"
 
-#ifndef ADAMW_CHUNK
-#define ADAMW_CHUNK 4096
-#endif                        // elements per workgroup of 256 threads
+#define ADAMW_CHUNK 2048      // elements per workgroup of 256 threads: one vector of eight per thread
 #define ADAMW_BLOCK 256       // elements per 8-bit block
 #define ADAMW_MAX_GRADS 480   // tensors per launch: the gradients' addresses travel in the kernel arguments (4 KB at most)
 #define ADAMW_MAX_GROUPS 48   // parameter groups per hyper launch (56 bytes each) and
@@ -110,15 +108,11 @@ __device__ __forceinline__ void adamw_st8(T* p, long long i, long long n, const 
 // ---------------------------------------------------------------------------------
 template <typename T, bool FULL>
 __device__ __forceinline__ double adamw_sumsq_chunk(const T* g, long long n, long long base) {
-  constexpr int IT = ADAMW_CHUNK / 2048;
-  float x[IT][8];
+  float x[8];
   double s[4] = {0.0, 0.0, 0.0, 0.0};
+  adamw_ld8<T, FULL>(g, base + threadIdx.x * 8, n, x);
 #pragma unroll
-  for (int it = 0; it < IT; ++it) adamw_ld8<T, FULL>(g, base + it * 2048 + threadIdx.x * 8, n, x[it]);
-#pragma unroll
-  for (int it = 0; it < IT; ++it)
-#pragma unroll
-    for (int e = 0; e < 8; ++e) s[e & 3] += (double)x[it][e] * (double)x[it][e];
+  for (int e = 0; e < 8; ++e) s[e & 3] += (double)x[e] * (double)x[e];
   return (s[0] + s[1]) + (s[2] + s[3]);
 }
 __global__ __launch_bounds__(256) void adamw_norm_kernel(AdamwGrads grads, const AdamwTensor* __restrict__ tensors, const int2* __restrict__ chunks,
@@ -186,25 +180,22 @@ template <typename T, bool FULL>
 __device__ __forceinline__ void adamw32_chunk(T* __restrict__ p, const T* __restrict__ g, float* __restrict__ m, float* __restrict__ v, long long n,
                                               long long base, const AdamwHyper& h) {
   const float b1 = (float)h.b1, c1 = (float)(h.c1 * h.coef), b2 = (float)h.b2, c2 = (float)(h.c2 * h.coef * h.coef);
+  const long long i = base + threadIdx.x * 8;
+  if (!FULL && i >= n) return;
+  float pv[8], gv[8], mv[8], vv[8];
+  adamw_ld8<T, FULL>(p, i, n, pv);
+  adamw_ld8<T, FULL>(g, i, n, gv);
+  ld8(m + i, mv);                       // the flat moment buffers are padded to whole blocks: zero behind the tensor, and zero they stay
+  ld8(v + i, vv);
 #pragma unroll
-  for (int it = 0; it < ADAMW_CHUNK / 2048; ++it) {
-    const long long i = base + it * 2048 + threadIdx.x * 8;
-    if (!FULL && i >= n) return;
-    float pv[8], gv[8], mv[8], vv[8];
-    adamw_ld8<T, FULL>(p, i, n, pv);
-    adamw_ld8<T, FULL>(g, i, n, gv);
-    ld8(m + i, mv);                       // the flat moment buffers are padded to whole blocks: zero behind the tensor, and zero they stay
-    ld8(v + i, vv);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      mv[e] = b1 * mv[e] + c1 * gv[e];
-      vv[e] = b2 * vv[e] + c2 * gv[e] * gv[e];
-      pv[e] = pv[e] * h.decay - h.step * mv[e] / (sqrtf(vv[e]) * h.isbc2 + h.eps);
-    }
-    adamw_st8<T, FULL>(p, i, n, pv);
-    st8(m + i, mv);
-    st8(v + i, vv);
+  for (int e = 0; e < 8; ++e) {
+    mv[e] = b1 * mv[e] + c1 * gv[e];
+    vv[e] = b2 * vv[e] + c2 * gv[e] * gv[e];
+    pv[e] = pv[e] * h.decay - h.step * mv[e] / (sqrtf(vv[e]) * h.isbc2 + h.eps);
   }
+  adamw_st8<T, FULL>(p, i, n, pv);
+  st8(m + i, mv);
+  st8(v + i, vv);
 }
 __global__ __launch_bounds__(256) void adamw32_kernel(AdamwGrads grads, const AdamwTensor* __restrict__ tensors, const int2* __restrict__ chunks,
                                                       const AdamwHyper* __restrict__ hyper, float* __restrict__ m, float* __restrict__ v,
@@ -251,77 +242,74 @@ template <typename T, bool FULL>
 __device__ __forceinline__ void adamw8_chunk(T* __restrict__ p, const T* __restrict__ g, uint8_t* __restrict__ mc, uint8_t* __restrict__ vc,
                                              float* __restrict__ ms, float* __restrict__ vs, long long n, long long base, const AdamwHyper& h) {
 #pragma clang fp contract(off)
-#pragma unroll 1
-  for (int it = 0; it < ADAMW_CHUNK / 2048; ++it) {
-    const long long blk = (base + it * 2048) / ADAMW_BLOCK + (threadIdx.x >> 5);
-    const long long i = blk * ADAMW_BLOCK + (threadIdx.x & 31) * 8;
-    if (!FULL && blk * ADAMW_BLOCK >= n) return;     // (uniform over the block's 32 lanes)
-    float pv[8], gv[8];
-    adamw_ld8<T, FULL>(p, i, n, pv);
-    adamw_ld8<T, FULL>(g, i, n, gv);
-    uint2 mq = *reinterpret_cast<const uint2*>(mc + i), vq = *reinterpret_cast<const uint2*>(vc + i);
-    const double am = (double)ms[blk] * (1.0 / 16129.0), av = (double)vs[blk] * (1.0 / (65025.0 * 65025.0));
-    mq.x ^= 0x80808080u; mq.y ^= 0x80808080u;        // signed bytes + 128: the byte conversions are unsigned
-    double m[8], v[8];
-    unsigned mx = 0, vx = 0;
+  const long long blk = base / ADAMW_BLOCK + (threadIdx.x >> 5);
+  const long long i = blk * ADAMW_BLOCK + (threadIdx.x & 31) * 8;
+  if (!FULL && blk * ADAMW_BLOCK >= n) return;     // (uniform over the block's 32 lanes)
+  float pv[8], gv[8];
+  adamw_ld8<T, FULL>(p, i, n, pv);
+  adamw_ld8<T, FULL>(g, i, n, gv);
+  uint2 mq = *reinterpret_cast<const uint2*>(mc + i), vq = *reinterpret_cast<const uint2*>(vc + i);
+  const double am = (double)ms[blk] * (1.0 / 16129.0), av = (double)vs[blk] * (1.0 / (65025.0 * 65025.0));
+  mq.x ^= 0x80808080u; mq.y ^= 0x80808080u;        // signed bytes + 128: the byte conversions are unsigned
+  double m[8], v[8];
+  unsigned mx = 0, vx = 0;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float km = (float)((e < 4 ? mq.x : mq.y) >> (8 * (e & 3)) & 255u) - 128.f, kv = (float)((e < 4 ? vq.x : vq.y) >> (8 * (e & 3)) & 255u);
-      const double gd = (double)gv[e] * h.coef, kv2 = (double)(kv * kv);
-      m[e] = h.b1 * ((double)(km * fabsf(km)) * am) + h.c1 * gd;
-      v[e] = h.b2 * (kv2 * kv2 * av) + h.c2 * gd * gd;
-      mx = max(mx, __float_as_uint((float)m[e]) & 0x7fffffffu);
-      vx = max(vx, __float_as_uint((float)v[e]) & 0x7fffffffu);
-    }
-    // one-instruction root and reciprocal (1 ulp each) unless eps is so small that a subnormal root would matter
-    if (h.eps >= 1e-12f) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-        pv[e] = pv[e] * h.decay - h.step * (float)m[e] * __builtin_amdgcn_rcpf(__builtin_amdgcn_sqrtf((float)v[e]) * h.isbc2 + h.eps);
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) pv[e] = pv[e] * h.decay - h.step * (float)m[e] / (sqrtf((float)v[e]) * h.isbc2 + h.eps);
-    }
-    adamw_st8<T, FULL>(p, i, n, pv);
-    mx = adamw_max32(mx);
-    vx = adamw_max32(vx);
-    // a block with a non-finite moment gets a NaN scale (its moments read back as NaN, as fp32 moments would stay); an empty one the scale 0; codes 0 for both.
-    // Scales whose reciprocal is out of fp32's range go through fp64.
-    const bool mbad = mx >= 0x7f800000u, vbad = vx >= 0x7f800000u;
-    const float sm = __uint_as_float(mx), sv = __uint_as_float(vx);
-    float km[8], kv[8];
-    if (!mbad && mx && sm < 1e-28f) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) km[e] = fminf((float)floor(127.0 * sqrt(fabs(m[e]) / (double)sm) + 0.5), 127.f);
-    } else {
-      const float inv = 16129.f / sm;
-      const double border = (double)sm * (1.0 / 16129.0);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) km[e] = adamw_code_m(m[e], inv, border);
-    }
-    if (!vbad && vx && sv < 1e-28f) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) kv[e] = fmaxf(fminf((float)floor(255.0 * sqrt(sqrt(v[e] / (double)sv)) + 0.5), 255.f), v[e] > 0.0 ? 1.f : 0.f);
-    } else {
-      const float inv = 65025.f * 65025.f / sv;
-      const double border = (double)sv * (1.0 / (65025.0 * 65025.0));
-#pragma unroll
-      for (int e = 0; e < 8; ++e) kv[e] = adamw_code_v(v[e], inv, border);
-    }
-    mq = vq = make_uint2(0, 0);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float biased = copysignf(km[e], (float)m[e]) + 128.f;
-      if (e < 4) { mq.x = __builtin_amdgcn_cvt_pk_u8_f32(biased, e, mq.x); vq.x = __builtin_amdgcn_cvt_pk_u8_f32(kv[e], e, vq.x); }
-      else { mq.y = __builtin_amdgcn_cvt_pk_u8_f32(biased, e - 4, mq.y); vq.y = __builtin_amdgcn_cvt_pk_u8_f32(kv[e], e - 4, vq.y); }
-    }
-    const bool mlive = !mbad && mx, vlive = !vbad && vx;
-    mq.x = mlive ? mq.x ^ 0x80808080u : 0; mq.y = mlive ? mq.y ^ 0x80808080u : 0;
-    vq.x = vlive ? vq.x : 0; vq.y = vlive ? vq.y : 0;
-    *reinterpret_cast<uint2*>(mc + i) = mq;
-    *reinterpret_cast<uint2*>(vc + i) = vq;
-    if ((threadIdx.x & 31) == 0) { ms[blk] = mbad ? NAN : sm; vs[blk] = vbad ? NAN : sv; }
+  for (int e = 0; e < 8; ++e) {
+    const float km = (float)((e < 4 ? mq.x : mq.y) >> (8 * (e & 3)) & 255u) - 128.f, kv = (float)((e < 4 ? vq.x : vq.y) >> (8 * (e & 3)) & 255u);
+    const double gd = (double)gv[e] * h.coef, kv2 = (double)(kv * kv);
+    m[e] = h.b1 * ((double)(km * fabsf(km)) * am) + h.c1 * gd;
+    v[e] = h.b2 * (kv2 * kv2 * av) + h.c2 * gd * gd;
+    mx = max(mx, __float_as_uint((float)m[e]) & 0x7fffffffu);
+    vx = max(vx, __float_as_uint((float)v[e]) & 0x7fffffffu);
   }
+  // one-instruction root and reciprocal (1 ulp each) unless eps is so small that a subnormal root would matter
+  if (h.eps >= 1e-12f) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      pv[e] = pv[e] * h.decay - h.step * (float)m[e] * __builtin_amdgcn_rcpf(__builtin_amdgcn_sqrtf((float)v[e]) * h.isbc2 + h.eps);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) pv[e] = pv[e] * h.decay - h.step * (float)m[e] / (sqrtf((float)v[e]) * h.isbc2 + h.eps);
+  }
+  adamw_st8<T, FULL>(p, i, n, pv);
+  mx = adamw_max32(mx);
+  vx = adamw_max32(vx);
+  // a block with a non-finite moment gets a NaN scale (its moments read back as NaN, as fp32 moments would stay); an empty one the scale 0; codes 0 for both.
+  // Scales whose reciprocal is out of fp32's range go through fp64.
+  const bool mbad = mx >= 0x7f800000u, vbad = vx >= 0x7f800000u;
+  const float sm = __uint_as_float(mx), sv = __uint_as_float(vx);
+  float km[8], kv[8];
+  if (!mbad && mx && sm < 1e-28f) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) km[e] = fminf((float)floor(127.0 * sqrt(fabs(m[e]) / (double)sm) + 0.5), 127.f);
+  } else {
+    const float inv = 16129.f / sm;
+    const double border = (double)sm * (1.0 / 16129.0);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) km[e] = adamw_code_m(m[e], inv, border);
+  }
+  if (!vbad && vx && sv < 1e-28f) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) kv[e] = fmaxf(fminf((float)floor(255.0 * sqrt(sqrt(v[e] / (double)sv)) + 0.5), 255.f), v[e] > 0.0 ? 1.f : 0.f);
+  } else {
+    const float inv = 65025.f * 65025.f / sv;
+    const double border = (double)sv * (1.0 / (65025.0 * 65025.0));
+#pragma unroll
+    for (int e = 0; e < 8; ++e) kv[e] = adamw_code_v(v[e], inv, border);
+  }
+  mq = vq = make_uint2(0, 0);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const float biased = copysignf(km[e], (float)m[e]) + 128.f;
+    if (e < 4) { mq.x = __builtin_amdgcn_cvt_pk_u8_f32(biased, e, mq.x); vq.x = __builtin_amdgcn_cvt_pk_u8_f32(kv[e], e, vq.x); }
+    else { mq.y = __builtin_amdgcn_cvt_pk_u8_f32(biased, e - 4, mq.y); vq.y = __builtin_amdgcn_cvt_pk_u8_f32(kv[e], e - 4, vq.y); }
+  }
+  const bool mlive = !mbad && mx, vlive = !vbad && vx;
+  mq.x = mlive ? mq.x ^ 0x80808080u : 0; mq.y = mlive ? mq.y ^ 0x80808080u : 0;
+  vq.x = vlive ? vq.x : 0; vq.y = vlive ? vq.y : 0;
+  *reinterpret_cast<uint2*>(mc + i) = mq;
+  *reinterpret_cast<uint2*>(vc + i) = vq;
+  if ((threadIdx.x & 31) == 0) { ms[blk] = mbad ? NAN : sm; vs[blk] = vbad ? NAN : sv; }
 }
 __global__ __launch_bounds__(256) void adamw8_kernel(AdamwGrads grads, const AdamwTensor* __restrict__ tensors, const int2* __restrict__ chunks,
                                                      const AdamwHyper* __restrict__ hyper, uint8_t* __restrict__ m, uint8_t* __restrict__ v,

@@ -15,7 +15,7 @@ import torch
 from . import _lib
 
 BLOCK = 256          # elements that share a scale of the 8-bit moments; every tensor starts at a multiple of it in the moment buffers
-CHUNK = 4096         # elements per workgroup (ADAMW_CHUNK of csrc/optim.cuh)
+CHUNK = 2048         # elements per workgroup (ADAMW_CHUNK of csrc/optim.cuh)
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _TABLE = np.dtype([("n", "<i8"), ("off", "<i8"), ("p", "<u8"), ("group", "<i4"), ("dt", "<i4")])      # MpmaeAdamwTensor
 
@@ -88,12 +88,19 @@ class _Plan:
         """Both moments as flat fp32 buffers: the state itself (32 bits) or what its codes stand for (8 bits)."""
         if self.bits == 32:
             return self.m, self.v
-        m, v = (torch.empty(self.size, dtype=torch.float32, device=self.device) for _ in range(2))
-        with torch.cuda.device(self.device):
-            err = _lib.load().mpmae_adamw_values(self.m.data_ptr(), self.v.data_ptr(), self.ms.data_ptr(), self.vs.data_ptr(), m.data_ptr(),
-                                                 v.data_ptr(), self.size, torch.cuda.current_stream(self.device).cuda_stream)
-        _lib.check(err, "adamw_values")
+        m, v = torch.empty(self.size, dtype=torch.float32, device=self.device), torch.empty(self.size, dtype=torch.float32, device=self.device)
+        a = self.args
+        self.launch("adamw_values", lambda stream: _lib.load().mpmae_adamw_values(a.m, a.v, a.ms, a.vs, m.data_ptr(), v.data_ptr(), self.size, stream))
         return m, v
+
+    def launch(self, what, call):
+        """call(stream) with this plan's device as the current one."""
+        if torch._C._cuda_getDevice() == self.device.index:
+            err = call(torch._C._cuda_getCurrentRawStream(self.device.index))
+        else:
+            with torch.cuda.device(self.device):
+                err = call(torch._C._cuda_getCurrentRawStream(self.device.index))
+        _lib.check(err, what)
 
     def store(self, m, v):
         """The inverse: flat fp32 moments into the state."""
@@ -258,16 +265,8 @@ class AdamW(torch.optim.Optimizer):
                 raise ValueError("lr is a number: a tensor would have to be read back on every step")
             groups += (g["lr"], *g["betas"], g["eps"], g["weight_decay"])
         hyper = (C.c_double * len(groups))(*groups)
-        if torch.cuda.current_device() == plan.device.index:
-            err = self._launch(plan, hyper)
-        else:
-            with torch.cuda.device(plan.device):
-                err = self._launch(plan, hyper)
-        _lib.check(err, "adamw_multi")
+        plan.launch("adamw_multi", lambda stream: _lib.load().mpmae_adamw_multi(plan.ref, plan.grads_at, hyper, len(self.param_groups), stream))
         return loss
-
-    def _launch(self, plan, hyper):
-        return _lib.load().mpmae_adamw_multi(plan.ref, plan.grads_at, hyper, len(hyper) // 5, torch.cuda.current_stream(plan.device).cuda_stream)
 
     # ---- checkpoints: torch.optim.AdamW's layout -------------------------------------------------------------------------------------------
     def state_dict(self):
