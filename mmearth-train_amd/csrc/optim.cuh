@@ -215,8 +215,7 @@ __global__ __launch_bounds__(256) void adamw32_kernel(AdamwGrads grads, const Ad
 
 // ---------------------------------------------------------------------------------
 // 8-bit moments. A lane holds eight consecutive elements, 32 lanes a block: the block's maxima are five lane exchanges. The moments are formed in fp64
-// (full rate on this machine) and the codes decided on them: the fp32 estimate of a code is exact except next to a border, where the border itself is
-// compared in fp64. Each fp64 operation rounds on its own, in the order of the formula (no contraction): a block's scale is often an exact tie between
+// (full rate on this machine) and the codes decided on them (adamw_codes_m / _v). Each fp64 operation rounds on its own, in the order of the formula (no contraction): a block's scale is often an exact tie between
 // two fp32 numbers ((9 s + g) / 10), and the scale, and with it every code, must not depend on how a compiler groups the terms.
 // ---------------------------------------------------------------------------------
 __device__ __forceinline__ unsigned adamw_max32(unsigned x) {      // maximum over the 32 lanes of a half wave (bit patterns of non-negative floats)
@@ -227,16 +226,47 @@ __device__ __forceinline__ unsigned adamw_max32(unsigned x) {      // maximum ov
   const auto y = __builtin_amdgcn_permlane16_swap(x, x, false, false);                // rows of 16: {0 0 2 2}, {1 1 3 3}
   return max(y[0], y[1]);
 }
-// The code next to a value. t: the code's fp32 estimate (off by less than 1e-3, so its whole part is at most one below); the border above that whole part is
-// compared in fp64. m: |m| >= (f + 1/2)^2 s / 127^2; the square is exact in fp32. v: v >= (f + 1/2)^4 s / 255^4.
-__device__ __forceinline__ float adamw_code_m(double m, float inv, double border) {       // |code|, 0..127
-  const float f = floorf(__builtin_amdgcn_sqrtf(fabsf((float)m) * inv)), b = f + 0.5f;
-  return fminf(f + (fabs(m) >= (double)(b * b) * border ? 1.f : 0.f), 127.f);
+// Codes of eight moments. Their fp32 estimates t = 127 sqrt(|m| / s), 255 (v / s)^(1/4) are off by less than 6e-5 (relative errors: 1.5 ulp of the quotient, halved
+// by each root, 1 ulp of each root), so rounding one is certain unless it lies within 1e-4 of a half; then the whole vector is decided on the border above
+// the estimate's whole part, in fp64: |m| >= (f + 1/2)^2 s / 127^2, v >= (f + 1/2)^4 s / 255^4 (the square is exact in fp32).
+__device__ __forceinline__ void adamw_codes_m(const double (&m)[8], float s, float (&k)[8]) {       // |codes|, 0..127
+  const float inv = 16129.f / s;
+  float near = 1.f;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const float t = __builtin_amdgcn_sqrtf(fabsf((float)m[e]) * inv), f = floorf(t), r = t - f;
+    near = fminf(near, fabsf(r - 0.5f));
+    k[e] = fminf(rintf(t), 127.f);
+  }
+  if (near < 1e-4f) {
+    const double border = (double)s * (1.0 / 16129.0);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float f = floorf(__builtin_amdgcn_sqrtf(fabsf((float)m[e]) * inv)), b = f + 0.5f;
+      k[e] = fminf(f + (fabs(m[e]) >= (double)(b * b) * border ? 1.f : 0.f), 127.f);
+    }
+  }
 }
-__device__ __forceinline__ float adamw_code_v(double v, float inv, double border) {       // 0..255, at least 1 where v > 0
-  const float f = floorf(__builtin_amdgcn_sqrtf(__builtin_amdgcn_sqrtf((float)v * inv))), b = f + 0.5f;
-  const double b2 = (double)(b * b);
-  return fmaxf(fminf(f + (v >= b2 * b2 * border ? 1.f : 0.f), 255.f), v > 0.0 ? 1.f : 0.f);
+__device__ __forceinline__ void adamw_codes_v(const double (&v)[8], float s, float (&k)[8]) {       // 0..255, at least 1 where v > 0
+  const float inv = 65025.f * 65025.f / s;
+  float near = 1.f;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const float t = __builtin_amdgcn_sqrtf(__builtin_amdgcn_sqrtf((float)v[e] * inv)), f = floorf(t), r = t - f;
+    near = fminf(near, fabsf(r - 0.5f));
+    k[e] = fminf(rintf(t), 255.f);
+  }
+  if (near < 1e-4f) {
+    const double border = (double)s * (1.0 / (65025.0 * 65025.0));
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float f = floorf(__builtin_amdgcn_sqrtf(__builtin_amdgcn_sqrtf((float)v[e] * inv))), b = f + 0.5f;
+      const double b2 = (double)(b * b);
+      k[e] = fminf(f + (v[e] >= b2 * b2 * border ? 1.f : 0.f), 255.f);
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < 8; ++e) k[e] = fmaxf(k[e], v[e] > 0.0 ? 1.f : 0.f);
 }
 template <typename T, bool FULL>
 __device__ __forceinline__ void adamw8_chunk(T* __restrict__ p, const T* __restrict__ g, uint8_t* __restrict__ mc, uint8_t* __restrict__ vc,
@@ -283,19 +313,13 @@ __device__ __forceinline__ void adamw8_chunk(T* __restrict__ p, const T* __restr
 #pragma unroll
     for (int e = 0; e < 8; ++e) km[e] = fminf((float)floor(127.0 * sqrt(fabs(m[e]) / (double)sm) + 0.5), 127.f);
   } else {
-    const float inv = 16129.f / sm;
-    const double border = (double)sm * (1.0 / 16129.0);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) km[e] = adamw_code_m(m[e], inv, border);
+    adamw_codes_m(m, sm, km);
   }
   if (!vbad && vx && sv < 1e-28f) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) kv[e] = fmaxf(fminf((float)floor(255.0 * sqrt(sqrt(v[e] / (double)sv)) + 0.5), 255.f), v[e] > 0.0 ? 1.f : 0.f);
   } else {
-    const float inv = 65025.f * 65025.f / sv;
-    const double border = (double)sv * (1.0 / (65025.0 * 65025.0));
-#pragma unroll
-    for (int e = 0; e < 8; ++e) kv[e] = adamw_code_v(v[e], inv, border);
+    adamw_codes_v(v, sv, kv);
   }
   mq = vq = make_uint2(0, 0);
 #pragma unroll
