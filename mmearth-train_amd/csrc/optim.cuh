@@ -234,9 +234,9 @@ __device__ __forceinline__ void adamw_codes_m(const double (&m)[8], float s, flo
   float near = 1.f;
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
-    const float t = __builtin_amdgcn_sqrtf(fabsf((float)m[e]) * inv), f = floorf(t), r = t - f;
-    near = fminf(near, fabsf(r - 0.5f));
-    k[e] = fminf(rintf(t), 127.f);
+    const float t = __builtin_amdgcn_sqrtf(fabsf((float)m[e]) * inv);
+    near = fminf(near, fabsf(__builtin_amdgcn_fractf(t) - 0.5f));
+    k[e] = rintf(t);                              // (t <= 127 (1 + 1e-6))
   }
   if (near < 1e-4f) {
     const double border = (double)s * (1.0 / 16129.0);
@@ -249,24 +249,23 @@ __device__ __forceinline__ void adamw_codes_m(const double (&m)[8], float s, flo
 }
 __device__ __forceinline__ void adamw_codes_v(const double (&v)[8], float s, float (&k)[8]) {       // 0..255, at least 1 where v > 0
   const float inv = 65025.f * 65025.f / s;
-  float near = 1.f;
+  float near = 1.f, least = 255.f;
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
-    const float t = __builtin_amdgcn_sqrtf(__builtin_amdgcn_sqrtf((float)v[e] * inv)), f = floorf(t), r = t - f;
-    near = fminf(near, fabsf(r - 0.5f));
-    k[e] = fminf(rintf(t), 255.f);
+    const float t = __builtin_amdgcn_sqrtf(__builtin_amdgcn_sqrtf((float)v[e] * inv));
+    near = fminf(near, fabsf(__builtin_amdgcn_fractf(t) - 0.5f));
+    k[e] = rintf(t);
+    least = fminf(least, k[e]);
   }
-  if (near < 1e-4f) {
+  if (near < 1e-4f || least < 1.f) {
     const double border = (double)s * (1.0 / (65025.0 * 65025.0));
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       const float f = floorf(__builtin_amdgcn_sqrtf(__builtin_amdgcn_sqrtf((float)v[e] * inv))), b = f + 0.5f;
       const double b2 = (double)(b * b);
-      k[e] = fminf(f + (v[e] >= b2 * b2 * border ? 1.f : 0.f), 255.f);
+      k[e] = fmaxf(fminf(f + (v[e] >= b2 * b2 * border ? 1.f : 0.f), 255.f), v[e] > 0.0 ? 1.f : 0.f);
     }
   }
-#pragma unroll
-  for (int e = 0; e < 8; ++e) k[e] = fmaxf(k[e], v[e] > 0.0 ? 1.f : 0.f);
 }
 template <typename T, bool FULL>
 __device__ __forceinline__ void adamw8_chunk(T* __restrict__ p, const T* __restrict__ g, uint8_t* __restrict__ mc, uint8_t* __restrict__ vc,
@@ -296,7 +295,7 @@ __device__ __forceinline__ void adamw8_chunk(T* __restrict__ p, const T* __restr
   if (h.eps >= 1e-12f) {
 #pragma unroll
     for (int e = 0; e < 8; ++e)
-      pv[e] = pv[e] * h.decay - h.step * (float)m[e] * __builtin_amdgcn_rcpf(__builtin_amdgcn_sqrtf((float)v[e]) * h.isbc2 + h.eps);
+      pv[e] = __builtin_fmaf(-h.step * (float)m[e], __builtin_amdgcn_rcpf(__builtin_fmaf(__builtin_amdgcn_sqrtf((float)v[e]), h.isbc2, h.eps)), pv[e] * h.decay);
   } else {
 #pragma unroll
     for (int e = 0; e < 8; ++e) pv[e] = pv[e] * h.decay - h.step * (float)m[e] / (sqrtf((float)v[e]) * h.isbc2 + h.eps);
