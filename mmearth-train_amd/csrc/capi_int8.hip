@@ -31,7 +31,7 @@ static void skinny(const MpmaeI8Args& a, hipStream_t st) {
 }
 template <typename T, int BM, int BN, int WM, int WN, int BK, int ST>
 static void tiles(const MpmaeI8Args& a, int count, const I8Tiles& tl, hipStream_t st) {
-  LAUNCH((i8_tile_kernel<T, BM, BN, WM, WN, BK, ST, false>), dim3(count * tl.subm * tl.subn), dim3(WM * WN * 64), (BM + BN) * BK * ST, st, (const int8_t*)a.q,
+  LAUNCH((i8_tile_kernel<T, BM, BN, WM, WN, BK, ST, false>), dim3(count * tl.subm * tl.subn), dim3(WM * WN * 64), i8_tile_lds(BM, BN, BK, ST), st, (const int8_t*)a.q,
          (const float*)a.sx, a.w, a.sw, a.bias, (T*)a.y, a.ldy, a.M, a.N, a.ldq, tl, (int*)nullptr);
 }
 template <typename T, int BM, int BN, int WM, int WN, int BK, int ST>
@@ -60,7 +60,7 @@ static void linear_i8(const MpmaeI8Args& a, hipStream_t st) {
   if (i8_few(a.M, a.N)) return skinny<T, 1, 1, false>(a, st);
   if (splits > 1) {
     const int mt = cdiv(a.M, 32), nt = cdiv(a.N, 64);
-    LAUNCH((i8_tile_kernel<T, 32, 64, 2, 2, 128, 4, true>), dim3(mt * nt, splits), dim3(256), (32 + 64) * 128 * 4, st, (const int8_t*)a.q, (const float*)a.sx, a.w, a.sw,
+    LAUNCH((i8_tile_kernel<T, 32, 64, 2, 2, 128, 4, true>), dim3(mt * nt, splits), dim3(256), i8_tile_lds(32, 64, 128, 4), st, (const int8_t*)a.q, (const float*)a.sx, a.w, a.sw,
            a.bias, (T*)a.y, a.ldy, a.M, a.N, a.ldq, (I8Tiles{mt, nt, 0, 1, 1}), a.part);
     LAUNCH(i8_join_kernel<T>, dim3(grid1d((long long)a.M * a.N, 256, 4096)), dim3(256), 0, st, (const int*)a.part, splits, (const float*)a.sx, a.sw, a.bias, (T*)a.y,
            a.ldy, a.M, a.N);

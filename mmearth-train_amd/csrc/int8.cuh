@@ -286,15 +286,24 @@ __global__ __launch_bounds__(512) void i8_skinny_kernel(const T* __restrict__ x,
 // index is XORed with a function of the row, on the source address of the load and on the fragment read, so that 16 lanes that read one chunk of 16 rows
 // meet no bank twice. D[n][m] = W x^T over pairs of column tiles with interleaved rows: a lane ends with eight consecutive columns of a row.
 // ---------------------------------------------------------------------------------
+typedef __attribute__((ext_vector_type(4))) unsigned u32x4_t;
+__device__ __forceinline__ void i8_st16(void* p, uint4 v) { __builtin_nontemporal_store(__builtin_bit_cast(u32x4_t, v), reinterpret_cast<u32x4_t*>(p)); }
 template <typename T> struct I8Out;
-template <> struct I8Out<float> { static __device__ __forceinline__ void st8v(float* p, const float (&v)[8]) { st8(p, v); } };
-template <> struct I8Out<bf16_t> { static __device__ __forceinline__ void st8v(bf16_t* p, const float (&v)[8]) { st8(p, v); } };
+template <> struct I8Out<float> {
+  static __device__ __forceinline__ void st8v(float* p, const float (&v)[8]) {
+    i8_st16(p, make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])));
+    i8_st16(p + 4, make_uint4(__float_as_uint(v[4]), __float_as_uint(v[5]), __float_as_uint(v[6]), __float_as_uint(v[7])));
+  }
+};
+template <> struct I8Out<bf16_t> {
+  static __device__ __forceinline__ void st8v(bf16_t* p, const float (&v)[8]) { i8_st16(p, make_uint4(f2bf2(v[0], v[1]), f2bf2(v[2], v[3]), f2bf2(v[4], v[5]), f2bf2(v[6], v[7]))); }
+};
 template <> struct I8Out<_Float16> {
   static __device__ __forceinline__ void st8v(_Float16* p, const float (&v)[8]) {
     I8Io<_Float16>::h8 a;
 #pragma unroll
     for (int i = 0; i < 8; ++i) a[i] = (_Float16)v[i];
-    *reinterpret_cast<I8Io<_Float16>::h8*>(p) = a;
+    i8_st16(p, __builtin_bit_cast(uint4, a));
   }
 };
 typedef const __attribute__((address_space(1))) void* i8_gptr_t;
@@ -304,6 +313,7 @@ typedef __attribute__((address_space(3))) void* i8_lptr_t;
 template <int BK> __device__ __forceinline__ int i8_swz_a(int row) { return BK == 128 ? row & 7 : (row >> 2) & 3; }
 template <int BK> __device__ __forceinline__ int i8_swz_b(int row) { return BK == 128 ? ((row & 3) | (((row >> 3) & 1) << 2)) : ((row >> 2) & 3); }
 
+constexpr int i8_tile_lds(int bm, int bn, int bk, int st) { return (bm + bn) * bk * st + (bm + 2 * bn) * 4; }
 constexpr int i8_waves_per_simd(int lds, int waves) { return 160 * 1024 / lds * waves / 4 > 0 ? 160 * 1024 / lds * waves / 4 : 1; }
 struct I8Tiles {
   int mt, nt;              // tiles of the whole product, of BM * subm rows and BN * subn columns
@@ -311,12 +321,12 @@ struct I8Tiles {
 };
 
 template <typename T, int BM, int BN, int WM, int WN, int BK, int ST, bool SPLIT>
-__global__ __launch_bounds__(WM * WN * 64, i8_waves_per_simd((BM + BN) * BK * ST, WM * WN)) void i8_tile_kernel(
+__global__ __launch_bounds__(WM * WN * 64, i8_waves_per_simd(i8_tile_lds(BM, BN, BK, ST), WM * WN)) void i8_tile_kernel(
     const int8_t* __restrict__ A, const float* __restrict__ sa, const int8_t* __restrict__ B, const float* __restrict__ sb, const float* __restrict__ bias,
     T* __restrict__ y, long long ldy, int M, int N, int Kp, I8Tiles tl, int* __restrict__ part) {
   constexpr int NTH = WM * WN * 64, RCH = BK / 16, TM = BM / WM / 16, TN = BN / WN / 16, KS = BK / 64;
   constexpr int AB = BM * BK, BB = BN * BK, STAGE = AB + BB, LA = AB / 16 / NTH, LB = BB / 16 / NTH;
-  static_assert(AB % (16 * NTH) == 0 && BB % (16 * NTH) == 0 && TN % 2 == 0 && STAGE * ST <= 160 * 1024, "tile shape");
+  static_assert(AB % (16 * NTH) == 0 && BB % (16 * NTH) == 0 && TN % 2 == 0 && i8_tile_lds(BM, BN, BK, ST) <= 160 * 1024, "tile shape");
   extern __shared__ __attribute__((aligned(16))) unsigned char i8_smem[];
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, wm = w / WN, wn = w % WN, lr = lane & 15, lg = lane >> 4;
   // tile order: workgroup L runs on XCD L % 8, whose L2 is its own: every XCD gets a contiguous run of tiles, four row tiles by all column tiles at a time
@@ -380,8 +390,26 @@ __global__ __launch_bounds__(WM * WN * 64, i8_waves_per_simd((BM + BN) * BK * ST
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
   };
+  // scales and bias of the tile go to LDS under the first slabs: read at the end, they would stand in front of the stores of a short k
+  float* const ep = reinterpret_cast<float*>(i8_smem + STAGE * ST);       // [BM] scales of x, [BN] scales of W, [BN] bias
+  float ev[(BM + 2 * BN + NTH - 1) / NTH];
+  if constexpr (!SPLIT) {
+#pragma unroll
+    for (int i = 0; i < (BM + 2 * BN + NTH - 1) / NTH; ++i) {
+      const int j = i * NTH + tid;
+      const float* src = j < BM ? sa + min(m0 + j, M - 1) : j < BM + BN ? sb + min(n0 + j - BM, N - 1) : (bias ? bias : sb) + min(n0 + j - BM - BN, N - 1);
+      ev[i] = *src;
+    }
+  }
 #pragma unroll
   for (int s = 0; s < ST - 1; ++s) if (s < nk) dma(s, s);
+  if constexpr (!SPLIT) {
+#pragma unroll
+    for (int i = 0; i < (BM + 2 * BN + NTH - 1) / NTH; ++i) {
+      const int j = i * NTH + tid;
+      if (j < BM + 2 * BN) ep[j] = j < BM + BN || bias ? ev[i] : 0.f;
+    }
+  }
   int slot = 0;
   if constexpr (KS == 2 && I8_PIPE) {
     // the fragments of the next half slab are read under the products of the current one, across the barrier too
@@ -438,13 +466,13 @@ __global__ __launch_bounds__(WM * WN * 64, i8_waves_per_simd((BM + BN) * BK * ST
   for (int jp = 0; jp < TN / 2; ++jp) {
     const int col = n0 + wn * TN * 16 + jp * 32 + lg * 8;
     float s[8], c[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) { const int n = min(col + e, N - 1); s[e] = sb[n]; c[e] = bias ? bias[n] : 0.f; }
+    ld8(ep + BM + col - n0, s);
+    ld8(ep + BM + BN + col - n0, c);
 #pragma unroll
     for (int i = 0; i < TM; ++i) {
       const int row = m0 + wm * TM * 16 + i * 16 + lr;
       if (row >= M) continue;
-      const float sr = sa[row];
+      const float sr = ep[row - m0];
       float v[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[e] = (float)acc[i][2 * jp + (e >> 2)][e & 3] * sr * s[e] + c[e];

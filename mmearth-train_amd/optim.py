@@ -158,8 +158,9 @@ class AdamW(torch.optim.Optimizer):
         super().add_param_group(group)
         try:
             self._check_group(self.param_groups[-1])
-            seen, device = set(), None
-            for p in (p for g in self.param_groups for p in g["params"]):
+            seen = {id(p) for g in self.param_groups[:-1] for p in g["params"]}          # (torch refuses a parameter of another group, and warns of one given twice)
+            device = self.param_groups[0]["params"][0].device if self.param_groups[0]["params"] else None
+            for p in self.param_groups[-1]["params"]:
                 if id(p) in seen:
                     raise ValueError("a parameter appears twice")
                 seen.add(id(p))
@@ -169,7 +170,6 @@ class AdamW(torch.optim.Optimizer):
                     raise ValueError("a parameter's elements have to lie densely in memory, each once")
                 if p.device.type != "cuda":
                     raise ValueError(f"this optimizer runs on the GPU only: a parameter is on {p.device}")
-                device = device or p.device
                 if p.device != device:
                     raise ValueError(f"the parameters of one optimizer are on one device: {device} and {p.device}")
             self._check_apart()
@@ -304,12 +304,13 @@ class AdamW(torch.optim.Optimizer):
                 raise ValueError(f"loaded moments of shape {tuple(st['exp_avg'].shape)} for a parameter of shape {tuple(p.shape)}")
         for mine, g in zip(self.param_groups, groups):
             mine.update({k: v for k, v in g.items() if k in self.defaults or k not in _TORCH_ONLY})
-        into = [torch.zeros(plan.size, device=plan.device) for _ in range(2)]
-        for i, (p, o, st) in enumerate(zip(plan.params, plan.offsets, entries)):
-            if st is not None:
-                _view(into[0], o, p).copy_(st["exp_avg"])
-                _view(into[1], o, p).copy_(st["exp_avg_sq"])
-        plan.store(*into)
+        into = [plan.m.zero_(), plan.v.zero_()] if self.state_bits == 32 else [torch.zeros(plan.size, device=plan.device) for _ in range(2)]
+        for flat, key in zip(into, ("exp_avg", "exp_avg_sq")):
+            there = [(_view(flat, o, p), st[key]) for p, o, st in zip(plan.params, plan.offsets, entries) if st is not None]
+            if there:
+                torch._foreach_copy_(*map(list, zip(*there)))
+        if self.state_bits == 8:
+            plan.store(*into)
         plan.steps.copy_(torch.tensor([0 if st is None else int(float(st["step"])) for st in entries], dtype=torch.int32))
 
     def __getstate__(self):
@@ -321,6 +322,8 @@ _TORCH_ONLY = {"params", "amsgrad", "maximize", "foreach", "capturable", "differ
 
 def _dense(p):
     """Whether the elements fill one stretch of memory, each once, in some order of the dimensions."""
+    if p.is_contiguous():
+        return True
     at = 1
     for size, stride in sorted(((n, s) for n, s in zip(p.shape, p.stride()) if n != 1), key=lambda x: x[1]):
         if stride != at:
