@@ -105,6 +105,13 @@ PyObject* linear_i8(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     if (x.dim() < 1 || x.size(-1) != k) return PyErr_Format(PyExc_ValueError, "inputs end in %lld elements, the weight's", k);
     if (x.device() != q.device() || !x.device().is_cuda())
       return PyErr_Format(PyExc_ValueError, "the input is on %s, the weight on %s", x.device().str().c_str(), q.device().str().c_str());
+    const auto plain = [&](const at::Tensor& t, at::ScalarType type, int64_t numel) {
+      return t.device() == q.device() && t.scalar_type() == type && t.is_contiguous() && t.numel() == numel;
+    };
+    if (q.dim() != 2 || q.scalar_type() != at::kChar || !q.is_contiguous() || q.size(0) < 1 || q.size(1) % 128 || q.size(1) < k || k < 1 ||
+        !plain(scale, at::kFloat, q.size(0)) || (args[3] != Py_None && !plain(THPVariable_Unpack(args[3]), at::kFloat, q.size(0))) ||
+        (reinterpret_cast<uintptr_t>(q.data_ptr()) & 15))
+      return PyErr_Format(PyExc_ValueError, "a weight is what quantize_weight makes: int8 rows of a multiple of 128, fp32 scales and bias, contiguous");
     const int64_t n = q.size(0), kp = q.size(1);
     at::DimVector shape(x.sizes().begin(), x.sizes().end());
     shape.back() = n;

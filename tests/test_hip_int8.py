@@ -208,6 +208,12 @@ def test_refusals_on_the_device():
         assert linear_int8(x, p).shape == (2, 8)
     with pytest.raises(ValueError, match="bias"):
         quantize_weight(w, torch.zeros(9, device="cuda"))
+    from mmearth_train_amd.int8 import Int8Weight
+    q, f = p.q, p.scale
+    for bad in (Int8Weight(q.float(), f, None, 16), Int8Weight(q, f.half(), None, 16), Int8Weight(q, f[:7], None, 16), Int8Weight(q[:, :100], f, None, 16),
+                Int8Weight(q[:, :64].contiguous(), f, None, 16), Int8Weight(q, f, f.double(), 16), Int8Weight(q, f.cpu(), None, 16)):
+        with pytest.raises(ValueError, match="quantize_weight makes"):
+            linear_int8(torch.zeros(2, 16, device="cuda"), bad)
 
 
 def test_a_network_is_trained_with_8_bit_moments_and_served_in_int8(tmp_path):

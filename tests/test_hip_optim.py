@@ -309,6 +309,18 @@ def test_state_must_exist_before_a_capture():
             opt.step()
 
 
+@pytest.mark.parametrize("bits", [32, 8])
+def test_edges_of_the_settings(bits):
+    """betas of 0, eps of 0 and tiny, a decay, one element: the update of the definition."""
+    from mmearth_train_amd.optim import AdamW
+    for betas, eps in (((0.0, 0.0), 1e-8), ((0.9, 0.999), 0.0), ((0.9, 0.999), 1e-20), ((0.0, 0.5), 1e-3)):
+        params = params_of([1, 700], DT[:1], 18)
+        refs = [Ref(p, bits) for p in params]
+        opt = AdamW(params, lr=1e-3, betas=betas, eps=eps, weight_decay=0.3, state_bits=bits)
+        run_steps(opt, params, refs, 3)
+        check(opt, params, refs, bits)
+
+
 def test_own_stream_and_determinism():
     from mmearth_train_amd.optim import AdamW
     got = []
@@ -326,19 +338,23 @@ def test_own_stream_and_determinism():
     assert all(torch.equal(a, b) for a, b in zip(*got))
 
 
-def test_groups_added_later_and_schedulers():
+@pytest.mark.parametrize("bits", [32, 8])
+def test_groups_added_later_and_schedulers(bits):
     from mmearth_train_amd.optim import AdamW
     params = params_of([500, 300, 1000], DT[:1], 14)
-    refs = [Ref(p, 32) for p in params]
-    opt = AdamW(params[:2], lr=1e-3)
+    refs = [Ref(p, bits) for p in params]
+    opt = AdamW(params[:2], lr=1e-3, state_bits=bits)
     sched = torch.optim.lr_scheduler.StepLR(opt, 1, 0.5)
     run_steps(opt, params[:2], refs, 2)
     sched.step()
     assert opt.param_groups[0]["lr"] == 5e-4
     opt.add_param_group({"params": [params[2]], "lr": 1e-2})
     run_steps(opt, params, refs, 2)
-    check(opt, params, refs, 32)
+    check(opt, params, refs, bits)
     assert opt.plan.steps.tolist() == [4, 4, 2]
+    with pytest.raises(ValueError, match="more than one parameter group|twice"):
+        opt.add_param_group({"params": [params[0]]})
+    assert len(opt.param_groups) == 2
 
 
 def test_refusals_on_the_device():
@@ -362,6 +378,10 @@ def test_refusals_on_the_device():
     p.grad = None
     with pytest.raises(ValueError, match="another size"):
         opt.step()
+    e = torch.nn.Embedding(4, 4, sparse=True).cuda()
+    e(torch.tensor([1], device="cuda")).sum().backward()
+    with pytest.raises(ValueError, match="sparse"):
+        AdamW(e.parameters()).step()
     with pytest.raises(RuntimeError, match="max_norm"):
         opt.grad_norm
     with pytest.raises(TypeError, match="state_dict"):
