@@ -4,12 +4,12 @@
 #include <algorithm>
 using std::min;
 
-template <typename T, bool WHOLE>
-static void quant_rows(const T* x, long long ldx, int M, int K, int8_t* q, int ldq, float* scale, hipStream_t st) {
-#define I8_Q(TPR, NV) LAUNCH((i8_quant_kernel<T, TPR, NV, WHOLE>), dim3(min(cdiv(M, 256 / TPR), 1 << 20)), dim3(256), 0, st, x, ldx, M, K, q, ldq, scale)
+template <typename T, bool RAGGED>
+static void quant_rows_of(const T* x, long long ldx, int M, int K, int8_t* q, int ldq, float* scale, hipStream_t st) {
+#define I8_Q(TPR, NV) LAUNCH((i8_quant_kernel<T, TPR, NV, RAGGED>), dim3(min(cdiv(M, 256 / TPR), 1 << 20)), dim3(256), 0, st, x, ldx, M, K, q, ldq, scale)
   // a wave per row while four vectors per lane hold it, then a workgroup per row, then a workgroup that reads the row twice
-  if (ldq <= 512) I8_Q(64, 1);
-  else if (!WHOLE) I8_Q(256, 0);
+  if (K < 8) I8_Q(64, -1);
+  else if (ldq <= 512) I8_Q(64, 1);
   else if (ldq <= 1024) I8_Q(64, 2);
   else if (ldq <= 2048) I8_Q(64, 4);
   else if (ldq <= 4096) I8_Q(256, 2);
@@ -20,8 +20,8 @@ static void quant_rows(const T* x, long long ldx, int M, int K, int8_t* q, int l
 }
 template <typename T>
 static void quant_rows(const T* x, long long ldx, int M, int K, int8_t* q, int ldq, float* scale, hipStream_t st) {
-  if (i8_whole(x, ldx, K)) quant_rows<T, true>(x, ldx, M, K, q, ldq, scale, st);
-  else quant_rows<T, false>(x, ldx, M, K, q, ldq, scale, st);
+  if (K & 7) quant_rows_of<T, true>(x, ldx, M, K, q, ldq, scale, st);
+  else quant_rows_of<T, false>(x, ldx, M, K, q, ldq, scale, st);
 }
 template <typename T, int MT, int NT, bool FUSED>
 static void skinny(const MpmaeI8Args& a, hipStream_t st) {
@@ -51,8 +51,8 @@ static int i8_splits(int M, int N, int Kp) {
 template <typename T>
 static void linear_i8(const MpmaeI8Args& a, hipStream_t st) {
   // Up to 8 rows of a moderate length: one launch that quantises and multiplies (1 x 1024 -> 4096: 4.8 us; 7.2 us in two launches). A workgroup holds the rows in
-  // its registers; longer ones, and rows of no whole vectors, go through a launch of their own.
-  if (a.M <= 8 && i8_vectors(a.M, a.ldq) <= I8_KEPT && i8_whole((const T*)a.x, a.ldx, a.K)) return skinny<T, 1, 1, true>(a, st);
+  // its registers; longer ones go through a launch of their own.
+  if (a.M <= 8 && i8_vectors(a.M, a.ldq) <= I8_KEPT && a.K >= 8) return skinny<T, 1, 1, true>(a, st);
   quant_rows((const T*)a.x, a.ldx, a.M, a.K, a.q, a.ldq, a.sx, st);
   auto count = [&](int bm, int bn) { return (long long)cdiv(a.M, bm) * cdiv(a.N, bn); };
   const int splits = i8_splits(a.M, a.N, a.ldq);

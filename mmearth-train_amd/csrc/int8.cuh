@@ -5,7 +5,7 @@
 // The integer sums are exact, so neither the order of k nor a split of it changes a result. A row that holds NaN or infinity has the scale NaN and
 // codes 0: its outputs are NaN, the other rows are untouched. Rows of codes are padded with zeros to a multiple of I8_KPAD bytes.
 #pragma once
-#include "common.cuh"
+#include "vec8.cuh"
 #include <type_traits>
 
 #define I8_KPAD 128
@@ -14,43 +14,22 @@
 #endif
 typedef __attribute__((ext_vector_type(4))) int i32x4_t;
 
-template <typename T> struct I8Io;
-template <> struct I8Io<float> {
-  static __device__ __forceinline__ float ld(const float* p) { return *p; }
-  static __device__ __forceinline__ void ld8v(const float* p, float (&o)[8]) { ld8(p, o); }
-  static __device__ __forceinline__ void st(float* p, float v) { *p = v; }
-};
-template <> struct I8Io<bf16_t> {
-  static __device__ __forceinline__ float ld(const bf16_t* p) { return bf2f(*p); }
-  static __device__ __forceinline__ void ld8v(const bf16_t* p, float (&o)[8]) { ld8(p, o); }
-  static __device__ __forceinline__ void st(bf16_t* p, float v) { *p = f2bf(v); }
-};
-template <> struct I8Io<_Float16> {
-  typedef __attribute__((ext_vector_type(8))) _Float16 h8;
-  static __device__ __forceinline__ float ld(const _Float16* p) { return (float)*p; }
-  static __device__ __forceinline__ void ld8v(const _Float16* p, float (&o)[8]) {
-    const h8 a = *reinterpret_cast<const h8*>(p);
+// Eight elements of a row of at least eight from element i on: one load from a clamped address (a load behind a branch is waited for where the branch joins,
+// and a row's loads would go one after the other). What lies past K becomes 0. Where K is no multiple of eight (RAGGED) the vector that straddles the end is
+// replaced by `last`, which every lane loads, element by element, once per row.
+template <typename T> __device__ __forceinline__ Raw8<T> i8_ld8(const T* row, int i, int K) { return raw8_ld(row + min(i, K - 8)); }
+template <typename T, bool RAGGED>
+__device__ __forceinline__ void i8_last8(const T* row, int K, float (&last)[8]) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) o[i] = (float)a[i];
-  }
-  static __device__ __forceinline__ void st(_Float16* p, float v) { *p = (_Float16)v; }
-};
-// Eight elements of a row from element i on; those at or past K read as 0. WHOLE (16-byte aligned rows of a multiple of eight elements): one load from a
-// clamped address, zeroed afterwards - a load behind a branch is waited for where the branch joins, and a row's loads would go one after the other.
-template <typename T> __host__ __device__ __forceinline__ bool i8_whole(const T* x, long long ldx, int K) {
-  return ((((uintptr_t)x) | ((uintptr_t)ldx * sizeof(T))) & 15) == 0 && (K & 7) == 0;
+  for (int e = 0; e < 8; ++e) last[e] = RAGGED && (K & ~7) + e < K ? elem_ld(row + min((K & ~7) + e, K - 1)) : 0.f;
 }
-template <typename T, bool WHOLE>
-__device__ __forceinline__ void i8_ld8(const T* row, int i, int K, float (&o)[8]) {
-  if (WHOLE) {
-    I8Io<T>::ld8v(row + min(i, K - 8), o);
+template <typename T, bool RAGGED>
+__device__ __forceinline__ void i8_end8(int i, int K, const Raw8<T>& raw, const float (&last)[8], float (&o)[8]) {
+  raw8_unpack(raw, o);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) o[e] = i < K ? o[e] : 0.f;
-  } else {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) o[e] = I8Io<T>::ld(row + min(i + e, K - 1));
-#pragma unroll
-    for (int e = 0; e < 8; ++e) o[e] = i + e < K ? o[e] : 0.f;
+  for (int e = 0; e < 8; ++e) {
+    if (RAGGED) o[e] = i + 8 <= K ? o[e] : i == (K & ~7) ? last[e] : 0.f;
+    else o[e] = i < K ? o[e] : 0.f;
   }
 }
 // Eight codes. Adding 1.5 * 2^23 rounds x * (127 / a) to the nearest whole number (half to even) and leaves it, as a byte of two's complement, in the low
@@ -103,32 +82,38 @@ __device__ __forceinline__ unsigned i8_row_max(unsigned mx, unsigned* red) {    
   }
   return mx;
 }
-// Rows to codes, the row held in registers between the maximum and the codes (NV vectors of eight per thread; NV = 0: any length, the row is read twice).
+// Rows to codes, the row held in registers between the maximum and the codes (NV vectors of eight per thread; NV = 0: any length of at least
+// eight, the row is read twice; NV = -1: fewer than eight).
 // Bound by memory: sizeof(T) + 1 bytes per element.
-template <typename T, int TPR, int NV, bool WHOLE>
+template <typename T, int TPR, int NV, bool RAGGED>
 __device__ __forceinline__ void i8_quant_row(const T* row, int K, int8_t* out, int ldq, float* scale, int t, unsigned* red) {
-  constexpr int NR = NV ? NV : 1;
-  float v[NR][8];
+  constexpr int NR = NV > 0 ? NV : 1;
+  float v[NR][8], last[8];
   unsigned mx = 0;
-  if (NV) {
+  auto take = [&](const float (&x)[8]) {
 #pragma unroll
-    for (int j = 0; j < NR; ++j) i8_ld8<T, WHOLE>(row, (j * TPR + t) * 8, K, v[j]);
+    for (int e = 0; e < 8; ++e) mx = max(mx, __float_as_uint(x[e]) & 0x7fffffffu);
+  };
+  if (NV > 0) {
+    Raw8<T> raw[NR];
 #pragma unroll
-    for (int j = 0; j < NR; ++j)
+    for (int j = 0; j < NR; ++j) raw[j] = i8_ld8(row, (j * TPR + t) * 8, K);
+    i8_last8<T, RAGGED>(row, K, last);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) mx = max(mx, __float_as_uint(v[j][e]) & 0x7fffffffu);
+    for (int j = 0; j < NR; ++j) { i8_end8<T, RAGGED>((j * TPR + t) * 8, K, raw[j], last, v[j]); take(v[j]); }
+  } else if (NV < 0) {                              // rows of fewer than eight elements
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[0][e] = t == 0 && e < K ? elem_ld(row + min(e, K - 1)) : 0.f;
+    take(v[0]);
   } else {
-    for (int i = t * 8; i < K; i += TPR * 8) {
-      i8_ld8<T, WHOLE>(row, i, K, v[0]);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) mx = max(mx, __float_as_uint(v[0][e]) & 0x7fffffffu);
-    }
+    i8_last8<T, RAGGED>(row, K, last);
+    for (int i = t * 8; i < K; i += TPR * 8) { i8_end8<T, RAGGED>(i, K, i8_ld8(row, i, K), last, v[0]); take(v[0]); }
   }
   mx = i8_row_max<TPR>(mx, red);
   const bool live = mx < 0x7f800000u && mx;
   const I8Row rw = i8_row(mx);
   if (t == 0) *scale = i8_scale(mx);
-  if (NV) {
+  if (NV != 0) {
 #pragma unroll
     for (int j = 0; j < NR; ++j) {
       const int i = (j * TPR + t) * 8;
@@ -139,19 +124,19 @@ __device__ __forceinline__ void i8_quant_row(const T* row, int K, int8_t* out, i
   } else {
     for (int i = t * 8; i < ldq; i += TPR * 8) {
       uint2 c = make_uint2(0, 0);
-      i8_ld8<T, WHOLE>(row, i, K, v[0]);
+      i8_end8<T, RAGGED>(i, K, i8_ld8(row, i, K), last, v[0]);
       if (live) c = i8_codes<T>(v[0], rw);
       *reinterpret_cast<uint2*>(out + i) = c;
     }
   }
 }
-template <typename T, int TPR, int NV, bool WHOLE>
+template <typename T, int TPR, int NV, bool RAGGED>
 __global__ __launch_bounds__(256) void i8_quant_kernel(const T* __restrict__ x, long long ldx, int M, int K, int8_t* __restrict__ q, int ldq,
                                                        float* __restrict__ scale) {
   __shared__ unsigned red[4];
   const int t = threadIdx.x % TPR;
   for (int m = blockIdx.x * (256 / TPR) + threadIdx.x / TPR; m < M; m += gridDim.x * (256 / TPR)) {
-    i8_quant_row<T, TPR, NV, WHOLE>(x + (size_t)m * ldx, K, q + (size_t)m * ldq, ldq, scale + m, t, red);
+    i8_quant_row<T, TPR, NV, RAGGED>(x + (size_t)m * ldx, K, q + (size_t)m * ldq, ldq, scale + m, t, red);
     if (TPR == 256) __syncthreads();      // red is written again
   }
 }
@@ -169,18 +154,22 @@ __host__ __device__ __forceinline__ int i8_waves_per_row(int M) { return M > 4 ?
 __host__ __device__ __forceinline__ int i8_vectors(int M, int Kp) { return (Kp + 512 * i8_waves_per_row(M) - 1) / (512 * i8_waves_per_row(M)); }
 constexpr int I8_KEPT = 6;
 // A row's vectors, at most NV a lane, stay in registers between the maximum and the codes.
-template <typename T, int NV>
+template <typename T, int NV, bool RAGGED>
 __device__ __forceinline__ void i8_quant_kept(const T* __restrict__ x, long long ldx, int M, int K, int8_t* Al, int Kp, float* ssx, unsigned (*smax)[8]) {
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, wpr = i8_waves_per_row(M), r = w / wpr, part = w % wpr, step = wpr * 512, i0 = (part * 64 + lane) * 8;
   const T* row = x + (size_t)min(r, M - 1) * ldx;
-  float v[NV][8];
+  Raw8<T> raw[NV];
+  float v[NV][8], last[8];
 #pragma unroll
-  for (int u = 0; u < NV; ++u) i8_ld8<T, true>(row, i0 + u * step, K, v[u]);
+  for (int u = 0; u < NV; ++u) raw[u] = i8_ld8(row, i0 + u * step, K);
+  i8_last8<T, RAGGED>(row, K, last);
   unsigned mx = 0;
 #pragma unroll
-  for (int u = 0; u < NV; ++u)
+  for (int u = 0; u < NV; ++u) {
+    i8_end8<T, RAGGED>(i0 + u * step, K, raw[u], last, v[u]);
 #pragma unroll
     for (int e = 0; e < 8; ++e) mx = max(mx, __float_as_uint(v[u][e]) & 0x7fffffffu);
+  }
   mx = i8_row_max<64>(mx, nullptr);
   if (lane == 0) smax[r][part] = mx;
   __syncthreads();
@@ -230,8 +219,11 @@ __global__ __launch_bounds__(512) void i8_skinny_kernel(const T* __restrict__ x,
   };
   load_w(w);                                                // the first weights are on their way while x is quantised
   if (FUSED) {
-    if (i8_vectors(M, Kp) <= 2) i8_quant_kept<T, 2>(x, ldx, M, K, Al, Kp, ssx, smax);
-    else i8_quant_kept<T, I8_KEPT>(x, ldx, M, K, Al, Kp, ssx, smax);
+    const bool two = i8_vectors(M, Kp) <= 2;
+    if ((K & 7) && two) i8_quant_kept<T, 2, true>(x, ldx, M, K, Al, Kp, ssx, smax);
+    else if (K & 7) i8_quant_kept<T, I8_KEPT, true>(x, ldx, M, K, Al, Kp, ssx, smax);
+    else if (two) i8_quant_kept<T, 2, false>(x, ldx, M, K, Al, Kp, ssx, smax);
+    else i8_quant_kept<T, I8_KEPT, false>(x, ldx, M, K, Al, Kp, ssx, smax);
   }
   const int8_t* a[MT];
 #pragma unroll
@@ -276,7 +268,7 @@ __global__ __launch_bounds__(512) void i8_skinny_kernel(const T* __restrict__ x,
 #pragma unroll
     for (int v = 0; v < 8; ++v) sum += red[v * MT * NT * 256 + o];
     const int tile = o >> 8, m = (tile / NT) * 16 + ((o >> 4) & 15), n = n0 + (tile % NT) * 16 + (o & 15);
-    if (m < M && n < N) I8Io<T>::st(y + (size_t)m * ldy + n, (float)sum * (FUSED ? ssx[m] : sa[m]) * sb[n] + (bias ? bias[n] : 0.f));
+    if (m < M && n < N) elem_st(y + (size_t)m * ldy + n, (float)sum * (FUSED ? ssx[m] : sa[m]) * sb[n] + (bias ? bias[n] : 0.f));
   }
 }
 
@@ -286,26 +278,6 @@ __global__ __launch_bounds__(512) void i8_skinny_kernel(const T* __restrict__ x,
 // index is XORed with a function of the row, on the source address of the load and on the fragment read, so that 16 lanes that read one chunk of 16 rows
 // meet no bank twice. D[n][m] = W x^T over pairs of column tiles with interleaved rows: a lane ends with eight consecutive columns of a row.
 // ---------------------------------------------------------------------------------
-typedef __attribute__((ext_vector_type(4))) unsigned u32x4_t;
-__device__ __forceinline__ void i8_st16(void* p, uint4 v) { __builtin_nontemporal_store(__builtin_bit_cast(u32x4_t, v), reinterpret_cast<u32x4_t*>(p)); }
-template <typename T> struct I8Out;
-template <> struct I8Out<float> {
-  static __device__ __forceinline__ void st8v(float* p, const float (&v)[8]) {
-    i8_st16(p, make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])));
-    i8_st16(p + 4, make_uint4(__float_as_uint(v[4]), __float_as_uint(v[5]), __float_as_uint(v[6]), __float_as_uint(v[7])));
-  }
-};
-template <> struct I8Out<bf16_t> {
-  static __device__ __forceinline__ void st8v(bf16_t* p, const float (&v)[8]) { i8_st16(p, make_uint4(f2bf2(v[0], v[1]), f2bf2(v[2], v[3]), f2bf2(v[4], v[5]), f2bf2(v[6], v[7]))); }
-};
-template <> struct I8Out<_Float16> {
-  static __device__ __forceinline__ void st8v(_Float16* p, const float (&v)[8]) {
-    I8Io<_Float16>::h8 a;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) a[i] = (_Float16)v[i];
-    i8_st16(p, __builtin_bit_cast(uint4, a));
-  }
-};
 typedef const __attribute__((address_space(1))) void* i8_gptr_t;
 typedef __attribute__((address_space(3))) void* i8_lptr_t;
 
@@ -462,7 +434,8 @@ __global__ __launch_bounds__(WM * WN * 64, i8_waves_per_simd(i8_tile_lds(BM, BN,
     }
     return;
   }
-  const bool vec = ((((uintptr_t)y) | ((uintptr_t)ldy * sizeof(T))) & 15) == 0;
+  // y goes past the caches where its pieces of 64 bytes are whole (50176 x 512 -> 2048: 82 -> 76 us); pieces that straddle need the cache to be put together
+  const bool past = ((((uintptr_t)y) | ((uintptr_t)ldy * sizeof(T))) & 63) == 0;
 #pragma unroll
   for (int jp = 0; jp < TN / 2; ++jp) {
     const int col = n0 + wn * TN * 16 + jp * 32 + lg * 8;
@@ -478,10 +451,11 @@ __global__ __launch_bounds__(WM * WN * 64, i8_waves_per_simd(i8_tile_lds(BM, BN,
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[e] = (float)acc[i][2 * jp + (e >> 2)][e & 3] * sr * s[e] + c[e];
       T* out = y + (size_t)row * ldy + col;
-      if (vec && col + 8 <= N) I8Out<T>::st8v(out, v);
+      if (past && col + 8 <= N) vec8_st<T, true>(out, v);
+      else if (col + 8 <= N) vec8_st(out, v);
       else {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) if (col + e < N) I8Io<T>::st(out + e, v[e]);
+        for (int e = 0; e < 8; ++e) if (col + e < N) elem_st(out + e, v[e]);
       }
     }
   }
@@ -496,6 +470,6 @@ __global__ __launch_bounds__(256) void i8_join_kernel(const int* __restrict__ pa
     int sum = 0;
     for (int s = 0; s < splits; ++s) sum += part[(size_t)s * all + o];
     const int m = (int)(o / N), n = (int)(o - (long long)m * N);
-    I8Io<T>::st(y + (size_t)m * ldy + n, (float)sum * sa[m] * sb[n] + (bias ? bias[n] : 0.f));
+    elem_st(y + (size_t)m * ldy + n, (float)sum * sa[m] * sb[n] + (bias ? bias[n] : 0.f));
   }
 }

@@ -11,7 +11,7 @@
 //
 // Everything is bound by memory: 3 * sizeof(p) + 16 bytes per element (fp32 moments), 3 * sizeof(p) + 4 + 1/16 (8 bits).
 #pragma once
-#include "common.cuh"
+#include "vec8.cuh"
 
 #define ADAMW_CHUNK 2048      // elements per workgroup of 256 threads: one vector of eight per thread
 #define ADAMW_BLOCK 256       // elements per 8-bit block
@@ -51,50 +51,21 @@ __device__ __forceinline__ double adamw_block_sum(double x, double* red) {
   return s;
 }
 
-template <typename T> struct AdamwIo;
-template <> struct AdamwIo<float> {
-  static __device__ __forceinline__ float ld(const float* p) { return *p; }
-  static __device__ __forceinline__ void st(float* p, float v) { *p = v; }
-  static __device__ __forceinline__ void ld8v(const float* p, float (&o)[8]) { ld8(p, o); }
-  static __device__ __forceinline__ void st8v(float* p, const float (&o)[8]) { st8(p, o); }
-};
-template <> struct AdamwIo<bf16_t> {
-  static __device__ __forceinline__ float ld(const bf16_t* p) { return bf2f(*p); }
-  static __device__ __forceinline__ void st(bf16_t* p, float v) { *p = f2bf(v); }
-  static __device__ __forceinline__ void ld8v(const bf16_t* p, float (&o)[8]) { ld8(p, o); }
-  static __device__ __forceinline__ void st8v(bf16_t* p, const float (&o)[8]) { st8(p, o); }
-};
-template <> struct AdamwIo<_Float16> {
-  typedef __attribute__((ext_vector_type(8))) _Float16 h8;
-  static __device__ __forceinline__ float ld(const _Float16* p) { return (float)*p; }
-  static __device__ __forceinline__ void st(_Float16* p, float v) { *p = (_Float16)v; }
-  static __device__ __forceinline__ void ld8v(const _Float16* p, float (&o)[8]) {
-    const h8 a = *reinterpret_cast<const h8*>(p);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) o[i] = (float)a[i];
-  }
-  static __device__ __forceinline__ void st8v(_Float16* p, const float (&o)[8]) {
-    h8 a;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) a[i] = (_Float16)o[i];
-    *reinterpret_cast<h8*>(p) = a;
-  }
-};
-// Eight consecutive elements from i on; those at or past n read as 0 and are not written. FULL: all inside, 16-byte aligned. Loads are never behind a branch (one
+// Eight consecutive elements from i on; those at or past n read as 0 and are not written. FULL: all inside. Loads are never behind a branch (one
 // is waited for where the branch joins): a ragged tensor's come from clamped addresses.
 template <typename T, bool FULL>
 __device__ __forceinline__ void adamw_ld8(const T* p, long long i, long long n, float (&o)[8]) {
-  if (FULL) { AdamwIo<T>::ld8v(p + i, o); return; }
+  if (FULL) { vec8_ld(p + i, o); return; }
 #pragma unroll
-  for (int e = 0; e < 8; ++e) o[e] = AdamwIo<T>::ld(p + min(i + e, n - 1));
+  for (int e = 0; e < 8; ++e) o[e] = elem_ld(p + min(i + e, n - 1));
 #pragma unroll
   for (int e = 0; e < 8; ++e) o[e] = i + e < n ? o[e] : 0.f;
 }
 template <typename T, bool FULL>
 __device__ __forceinline__ void adamw_st8(T* p, long long i, long long n, const float (&o)[8]) {
-  if (FULL) { AdamwIo<T>::st8v(p + i, o); return; }
+  if (FULL) { vec8_st(p + i, o); return; }
 #pragma unroll
-  for (int e = 0; e < 8; ++e) if (i + e < n) AdamwIo<T>::st(p + i + e, o[e]);
+  for (int e = 0; e < 8; ++e) if (i + e < n) elem_st(p + i + e, o[e]);
 }
 // a workgroup's chunk in the form that its tensor allows
 #define ADAMW_BY_TYPE(...)                                                                        \
@@ -127,7 +98,7 @@ __global__ __launch_bounds__(256) void adamw_norm_kernel(AdamwGrads grads, const
     const void* g = grads.g[ch.x - grads.first];
     const long long base = (long long)ch.y * ADAMW_CHUNK;
     if (g) {
-      const bool full = (((uintptr_t)g) & 15) == 0 && base + ADAMW_CHUNK <= t.n;
+      const bool full = base + ADAMW_CHUNK <= t.n;
       ADAMW_BY_TYPE(s += full ? adamw_sumsq_chunk<T, true>((const T*)g, t.n, base) : adamw_sumsq_chunk<T, false>((const T*)g, t.n, base);)
     }
     ch = ch_next;
@@ -179,6 +150,7 @@ __global__ __launch_bounds__(512) void adamw_hyper_kernel(AdamwGroups groups, co
 template <typename T, bool FULL>
 __device__ __forceinline__ void adamw32_chunk(T* __restrict__ p, const T* __restrict__ g, float* __restrict__ m, float* __restrict__ v, long long n,
                                               long long base, const AdamwHyper& h) {
+#pragma clang fp contract(off)      // (the same bits whichever form a chunk takes)
   const float b1 = (float)h.b1, c1 = (float)(h.c1 * h.coef), b2 = (float)h.b2, c2 = (float)(h.c2 * h.coef * h.coef);
   const long long i = base + threadIdx.x * 8;
   if (!FULL && i >= n) return;
@@ -189,9 +161,9 @@ __device__ __forceinline__ void adamw32_chunk(T* __restrict__ p, const T* __rest
   ld8(v + i, vv);
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
-    mv[e] = b1 * mv[e] + c1 * gv[e];
-    vv[e] = b2 * vv[e] + c2 * gv[e] * gv[e];
-    pv[e] = pv[e] * h.decay - h.step * mv[e] / (sqrtf(vv[e]) * h.isbc2 + h.eps);
+    mv[e] = __builtin_fmaf(b1, mv[e], c1 * gv[e]);
+    vv[e] = __builtin_fmaf(b2, vv[e], c2 * gv[e] * gv[e]);
+    pv[e] = __builtin_fmaf(pv[e], h.decay, -(h.step * mv[e] / __builtin_fmaf(sqrtf(vv[e]), h.isbc2, h.eps)));
   }
   adamw_st8<T, FULL>(p, i, n, pv);
   st8(m + i, mv);
@@ -208,7 +180,7 @@ __global__ __launch_bounds__(256) void adamw32_kernel(AdamwGrads grads, const Ad
   if (!g || (norm_skip && norm_skip[1] != 0.f)) return;
   const AdamwHyper h = hyper[ch.x];
   const long long base = (long long)ch.y * ADAMW_CHUNK;
-  const bool full = ((((uintptr_t)p) | ((uintptr_t)g)) & 15) == 0 && base + ADAMW_CHUNK <= t.n;
+  const bool full = base + ADAMW_CHUNK <= t.n;
   ADAMW_BY_TYPE(if (full) adamw32_chunk<T, true>((T*)p, (const T*)g, m + t.off, v + t.off, t.n, base, h);
                 else adamw32_chunk<T, false>((T*)p, (const T*)g, m + t.off, v + t.off, t.n, base, h);)
 }
@@ -345,7 +317,7 @@ __global__ __launch_bounds__(256) void adamw8_kernel(AdamwGrads grads, const Ada
   if (!g || (norm_skip && norm_skip[1] != 0.f)) return;
   const AdamwHyper h = hyper[ch.x];
   const long long base = (long long)ch.y * ADAMW_CHUNK, sb = t.off / ADAMW_BLOCK;
-  const bool full = ((((uintptr_t)p) | ((uintptr_t)g)) & 15) == 0 && base + ADAMW_CHUNK <= t.n;
+  const bool full = base + ADAMW_CHUNK <= t.n;
   ADAMW_BY_TYPE(if (full) adamw8_chunk<T, true>((T*)p, (const T*)g, m + t.off, v + t.off, ms + sb, vs + sb, t.n, base, h);
                 else adamw8_chunk<T, false>((T*)p, (const T*)g, m + t.off, v + t.off, ms + sb, vs + sb, t.n, base, h);)
 }
