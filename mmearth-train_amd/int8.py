@@ -122,12 +122,17 @@ class Int8Linear(nn.Module):
         return f"in_features={self.in_features}, out_features={self.out_features}, bias={self.bias is not None}"
 
 
-def quantize_model(model):
-    """Every nn.Linear of the module tree (on the GPU) becomes an Int8Linear, in place; returns the model."""
-    if isinstance(model, nn.Linear):
-        return Int8Linear.from_linear(model)
-    for name, child in model.named_children():
-        new = quantize_model(child)
-        if new is not child:
-            setattr(model, name, new)
+def quantize_model(model, _made=None):
+    """Every nn.Linear of the module tree (on the GPU; no subclasses, whose users may read the weight) becomes an Int8Linear, in place; one that is used in
+    several places stays one. Returns the model."""
+    made = {} if _made is None else _made
+    if id(model) in made:
+        return made[id(model)]
+    made[id(model)] = model
+    if type(model) is nn.Linear:
+        made[id(model)] = Int8Linear.from_linear(model)
+        return made[id(model)]
+    for name, child in model._modules.items():
+        if child is not None:
+            model._modules[name] = quantize_model(child, made)
     return model

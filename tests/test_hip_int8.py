@@ -108,7 +108,7 @@ def test_leading_dimensions_strides_and_offsets():
     for dtype in DT.values():
         room = torch.randn(6, 5, 4, 200, device="cuda", generator=gen).to(dtype)
         for x in (room[..., :70], room[..., 3:73], room[2, 1, 0, 1:71], room[0, 0, :, 5:75], room.permute(3, 0, 1, 2)[:4, :, :, 0].new_tensor(0).expand(3, 70),
-                  room[0, 0, :, :70].t().contiguous().t(), room[:0, ..., :70], room[:, :, :, :70].transpose(0, 2)):
+                  room[0, 0, :, :70].t().contiguous().t(), room[:0, ..., :70], room[:, :, :, :70].transpose(0, 2), room[0, 0, :1, 2:72].expand(9, 70)):
             y = linear_int8(x, p)
             assert y.shape == x.shape[:-1] + (90,)
             if x.numel():
@@ -264,6 +264,29 @@ def test_a_network_is_trained_with_8_bit_moments_and_served_in_int8(tmp_path):
         lin = half.head
         assert lin.scale.dtype == torch.float32 and lin.q.dtype == torch.int8
         assert half(x.half()).dtype == torch.float16
+
+
+def test_shared_and_foreign_layers_of_a_model():
+    from mmearth_train_amd.int8 import Int8Linear, quantize_model
+
+    class Net(torch.nn.Module):
+        def __init__(self):
+            super().__init__()
+            self.a = torch.nn.Linear(16, 16)
+            self.b = self.a
+            self.c = torch.nn.Sequential(self.a, torch.nn.ReLU())
+            self.d = torch.nn.MultiheadAttention(16, 2)
+            self.e = None
+
+        def forward(self, x):
+            return self.c(self.b(self.a(x)))
+
+    net = quantize_model(Net().cuda())
+    assert isinstance(net.a, Int8Linear) and net.a is net.b and net.a is net.c[0]
+    assert not isinstance(net.d.out_proj, Int8Linear)
+    with torch.no_grad():
+        assert net(torch.randn(3, 16, device="cuda")).shape == (3, 16)
+        net.d(*[torch.randn(3, 1, 16, device="cuda")] * 3)
 
 
 def nn_loss(y, t):
