@@ -24,16 +24,27 @@ bool same_order(const at::Tensor& a, const at::Tensor& b) {
   return true;
 }
 
-// gather(params, table, device, out) -> (tensors with a gradient, whether a parameter has moved, None or [indices whose gradient lies in another element order])
+// what decides the order of a dense tensor's elements in memory
+uint64_t order_of(const at::Tensor& t) {
+  uint64_t h = 1469598103934665603ull;
+  const auto n = t.sizes(), s = t.strides();
+  for (size_t i = 0; i < n.size(); ++i)
+    if (n[i] != 1) h = ((h ^ (uint64_t)n[i]) * 1099511628211ull ^ (uint64_t)s[i]) * 1099511628211ull;
+  return h | 1;
+}
+
+// gather(params, table, device, out, orders, update) -> (tensors with a gradient, whether a parameter has moved, None or [indices whose gradient lies in another element order])
 // table: address of the host copy of MpmaeAdamwTensor[len(params)], whose parameter addresses are brought up to date; out: address of the gradients'
-// addresses, 0 where there is none.
+// addresses, 0 where there is none; orders: address of one word per parameter, 0 before the first call, that holds it to its element order (its moments lie
+// in the same); update: the parameters with a gradient are about to be written.
 PyObject* gather(PyObject*, PyObject* args) {
   PyObject* list;
-  unsigned long long expected_at, out_at;
-  int device;
-  if (!PyArg_ParseTuple(args, "O!KiK", &PyList_Type, &list, &expected_at, &device, &out_at)) return nullptr;
+  unsigned long long expected_at, out_at, orders_at;
+  int device, update;
+  if (!PyArg_ParseTuple(args, "O!KiKKp", &PyList_Type, &list, &expected_at, &device, &out_at, &orders_at, &update)) return nullptr;
   MpmaeAdamwTensor* want = reinterpret_cast<MpmaeAdamwTensor*>(expected_at);
   uint64_t* out = reinterpret_cast<uint64_t*>(out_at);
+  uint64_t* orders = reinterpret_cast<uint64_t*>(orders_at);
   PyObject* other = nullptr;
   try {
     const Py_ssize_t count = PyList_GET_SIZE(list);
@@ -48,7 +59,9 @@ PyObject* gather(PyObject*, PyObject* args) {
         if (p.layout() != at::kStrided || !p.device().is_cuda() || p.device().index() != device) wrong = "has left the optimizer's device";
         else if (p.numel() != want[i].n || code_of(p.scalar_type()) != want[i].dt) wrong = "has another size or type than when the optimizer first ran";
         else if (!p.is_non_overlapping_and_dense()) wrong = "is not dense in memory";
+        else if (const uint64_t order = order_of(p); orders[i] && orders[i] != order) wrong = "has its elements in another order than when the optimizer first ran";
         else {
+          orders[i] = order;
           const at::Tensor& g = p.grad();
           void* const at = p.data_ptr();
           moved |= want[i].p != at;
@@ -59,7 +72,7 @@ PyObject* gather(PyObject*, PyObject* args) {
             else if (g.device() != p.device() || g.scalar_type() != p.scalar_type() || g.sizes() != p.sizes()) wrong = "has a gradient of another device, type or shape";
             else {
               ++grads;
-              p.unsafeGetTensorImpl()->bump_version();      // the kernel writes it behind autograd's back: a stale saved tensor has to be noticed
+              if (update) p.unsafeGetTensorImpl()->bump_version();      // the kernel writes it behind autograd's back: a stale saved tensor has to be noticed
               if (same_order(p, g)) out[i] = reinterpret_cast<uint64_t>(g.data_ptr());
               else {
                 if (!other && !(other = PyList_New(0))) return nullptr;

@@ -61,7 +61,7 @@ class _Plan:
         chunks = np.empty((int(per.sum()), 2), np.int32)
         chunks[:, 0] = np.repeat(np.arange(nt), per)
         chunks[:, 1] = np.arange(len(chunks)) - np.repeat(self.chunk_first[:-1], per)
-        self.grads = np.zeros(nt, np.uint64)
+        self.grads, self.orders = np.zeros(nt, np.uint64), np.zeros(nt, np.uint64)
         new = lambda n, dtype: torch.zeros(n, dtype=dtype, device=device)  # noqa: E731
         self.d_table = torch.from_numpy(self.table.view(np.uint8).copy()).to(device)
         self.d_chunks = torch.from_numpy(chunks).to(device)
@@ -81,7 +81,8 @@ class _Plan:
                                    hyper=at(self.hyper), partials=at(self.partials), norm_skip=at(self.norm_skip), m=at(self.m), v=at(self.v),
                                    ms=at(self.ms), vs=at(self.vs), max_norm=float(max_norm or 0.0), nt=nt, npartials=npart, bits=bits)
         self.ref, self.stale = C.byref(self.args), False          # stale: parameters have moved and the device table does not know
-        self.table_at, self.grads_at = self.table.ctypes.data, self.grads.ctypes.data
+        self.table_at, self.grads_at, self.orders_at = self.table.ctypes.data, self.grads.ctypes.data, self.orders.ctypes.data
+        _lib.host_tensors().gather(params, self.table_at, device.index, self.grads_at, self.orders_at, False)      # (holds them to the order that offsets go by)
         torch.cuda.current_stream(device).synchronize()      # the tables and zeroed moments are there for whatever stream steps first
 
     def values(self):
@@ -159,7 +160,7 @@ class AdamW(torch.optim.Optimizer):
         try:
             self._check_group(self.param_groups[-1])
             seen = {id(p) for g in self.param_groups[:-1] for p in g["params"]}          # (torch refuses a parameter of another group, and warns of one given twice)
-            device = self.param_groups[0]["params"][0].device if self.param_groups[0]["params"] else None
+            device = next((p.device for g in self.param_groups for p in g["params"]), None)
             for p in self.param_groups[-1]["params"]:
                 if id(p) in seen:
                     raise ValueError("a parameter appears twice")
@@ -243,7 +244,7 @@ class AdamW(torch.optim.Optimizer):
             with torch.enable_grad():
                 loss = closure()
         plan = self.plan
-        grads, moved, other = _lib.host_tensors().gather(plan.params, plan.table_at, plan.device.index, plan.grads_at)
+        grads, moved, other = _lib.host_tensors().gather(plan.params, plan.table_at, plan.device.index, plan.grads_at, plan.orders_at, True)
         plan.stale |= moved
         if plan.stale:                                 # (`p.data = ...`, `model.load_state_dict(assign=True)`)
             if torch.cuda.is_current_stream_capturing():
@@ -304,11 +305,15 @@ class AdamW(torch.optim.Optimizer):
                 raise ValueError(f"loaded moments of shape {tuple(st['exp_avg'].shape)} for a parameter of shape {tuple(p.shape)}")
         for mine, g in zip(self.param_groups, groups):
             mine.update({k: v for k, v in g.items() if k in self.defaults or k not in _TORCH_ONLY})
-        into = [plan.m.zero_(), plan.v.zero_()] if self.state_bits == 32 else [torch.zeros(plan.size, device=plan.device) for _ in range(2)]
+        into = [plan.m, plan.v] if self.state_bits == 32 else [torch.zeros(plan.size, device=plan.device) for _ in range(2)]
         for flat, key in zip(into, ("exp_avg", "exp_avg_sq")):
-            there = [(_view(flat, o, p), st[key]) for p, o, st in zip(plan.params, plan.offsets, entries) if st is not None]
+            views = [_view(flat, o, p) for p, o in zip(plan.params, plan.offsets)]
+            there = [(view, st[key]) for view, st in zip(views, entries) if st is not None]
+            absent = [view for view, st in zip(views, entries) if st is None]
             if there:
                 torch._foreach_copy_(*map(list, zip(*there)))
+            if absent:
+                torch._foreach_zero_(absent)
         if self.state_bits == 8:
             plan.store(*into)
         plan.steps.copy_(torch.tensor([0 if st is None else int(float(st["step"])) for st in entries], dtype=torch.int32))

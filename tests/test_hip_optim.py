@@ -423,6 +423,9 @@ def test_autograd_notices_the_update():
     AdamW([w]).step()
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         y.backward()
+    y = (x @ w).sum()
+    AdamW([w]).flat_moments()                # (making the state writes no parameter)
+    y.backward()
 
 
 def test_a_step_beside_a_live_graph_of_the_same_leaves():
@@ -497,3 +500,45 @@ def test_parameters_that_move_in_memory():
     q.data = x[100:400]
     with pytest.raises(ValueError, match="share memory"):
         c.step()
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_another_element_order_is_refused(bits):
+    """The moments lie in the parameter's element order of the first step: a parameter that is laid out anew afterwards is not updated with misplaced ones."""
+    from mmearth_train_amd.optim import AdamW
+    w = torch.nn.Parameter(torch.randn(6, 4, 3, 3, device="cuda"))
+    w.grad = torch.randn_like(w)
+    opt = AdamW([w], state_bits=bits)
+    opt.step()
+    w.data = w.data.contiguous(memory_format=torch.channels_last)
+    before = w.detach().clone()
+    with pytest.raises(ValueError, match="another order"):
+        opt.step()
+    assert torch.equal(before, w)
+    w.data = w.data.contiguous()
+    opt.step()
+    assert opt.plan.steps.tolist() == [2]
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_loading_views_of_the_state_itself_and_lists_with_holes(bits):
+    from mmearth_train_amd.optim import AdamW
+    params = params_of([300, 700, 5], DT[:1], 19)
+    opt = AdamW([{"params": []}, {"params": params}], state_bits=bits)
+    grads_for(params, 1)
+    params[1].grad = None
+    opt.step()
+    sd = opt.state_dict()
+    assert sorted(sd["state"]) == [0, 2]
+    m, v = opt.flat_moments()
+    keep = m.clone(), v.clone()
+    for i in (0, 2):
+        o, n = opt.offsets[i], params[i].numel()
+        sd["state"][i]["exp_avg"], sd["state"][i]["exp_avg_sq"] = m[o:o + n], v[o:o + n]
+    opt.load_state_dict(sd)
+    assert all(torch.equal(a, b) for a, b in zip(keep, opt.flat_moments())) and opt.plan.steps.tolist() == [1, 0, 1]
+    grads_for(params, 2)
+    opt.step()
+    opt.load_state_dict(sd | {"state": {0: sd["state"][0]}})
+    m, v = opt.flat_moments()
+    assert not m[opt.offsets[1]:].any() and not v[opt.offsets[1]:].any() and opt.plan.steps.tolist() == [1, 0, 0]

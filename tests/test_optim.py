@@ -115,10 +115,10 @@ def test_native_reader_refuses_what_it_cannot_address():
     host = _lib.host_tensors()
     table, out = np.zeros(1, optim._TABLE), np.zeros(2, np.uint64)
     with pytest.raises(ValueError, match="device"):
-        host.gather([torch.nn.Parameter(torch.zeros(3))], table.ctypes.data, 0, out.ctypes.data)
+        host.gather([torch.nn.Parameter(torch.zeros(3))], table.ctypes.data, 0, out.ctypes.data, out.ctypes.data, True)
     with pytest.raises(ValueError, match="not a tensor"):
-        host.gather([3], table.ctypes.data, 0, out.ctypes.data)
-    assert host.gather([], table.ctypes.data, 0, out.ctypes.data) == (0, False, None)
+        host.gather([3], table.ctypes.data, 0, out.ctypes.data, out.ctypes.data, True)
+    assert host.gather([], table.ctypes.data, 0, out.ctypes.data, out.ctypes.data, True) == (0, False, None)
 
 
 @pytest.fixture(scope="module")
