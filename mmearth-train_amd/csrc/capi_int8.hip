@@ -7,8 +7,11 @@ using std::min;
 template <typename T, bool RAGGED>
 static void quant_rows_of(const T* x, long long ldx, int M, int K, int8_t* q, int ldq, float* scale, hipStream_t st) {
 #define I8_Q(TPR, NV) LAUNCH((i8_quant_kernel<T, TPR, NV, RAGGED>), dim3(min(cdiv(M, 256 / TPR), 1 << 20)), dim3(256), 0, st, x, ldx, M, K, q, ldq, scale)
-  // a wave per row while four vectors per lane hold it, then a workgroup per row, then a workgroup that reads the row twice
-  if (K < 8) I8_Q(64, -1);
+  // 16 or 32 lanes per short row (49050 x 18: a wave per row takes four times the waves), a wave per row while four vectors per lane hold it, then a workgroup per
+  // row, then a workgroup that reads the row twice
+  if (K < 8) I8_Q(16, -1);
+  else if (ldq <= 128) I8_Q(16, 1);
+  else if (ldq <= 256) I8_Q(32, 1);
   else if (ldq <= 512) I8_Q(64, 1);
   else if (ldq <= 1024) I8_Q(64, 2);
   else if (ldq <= 2048) I8_Q(64, 4);

@@ -76,9 +76,9 @@ __device__ __forceinline__ uint2 i8_codes(const float (&x)[8], const I8Row& row)
   return q;
 }
 template <int TPR>
-__device__ __forceinline__ unsigned i8_row_max(unsigned mx, unsigned* red) {      // over the TPR threads of a row; 64: one wave, 256: the workgroup
+__device__ __forceinline__ unsigned i8_row_max(unsigned mx, unsigned* red) {      // over the TPR threads of a row: part of a wave, a wave, or (256) the workgroup
 #pragma unroll
-  for (int d = 32; d; d >>= 1) mx = max(mx, (unsigned)__shfl_xor((int)mx, d));
+  for (int d = TPR < 64 ? TPR / 2 : 32; d; d >>= 1) mx = max(mx, (unsigned)__shfl_xor((int)mx, d));
   if (TPR == 256) {
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = mx;
     __syncthreads();
