@@ -76,7 +76,8 @@ def quantize_weight(weight, bias=None):
     with torch.cuda.device(weight.device):
         err = _lib.load().mpmae_quant_i8(_DTYPES[w.dtype], w.data_ptr(), ld, n, k, q.data_ptr(), kp, scale.data_ptr(), _stream(weight.device))
     _lib.check(err, "quant_i8")
-    return Int8Weight(q, scale, None if bias is None else bias.detach().float().contiguous(), k)
+    # (a copy of the bias too: the codes are those of this moment)
+    return Int8Weight(q, scale, None if bias is None else bias.detach().to(torch.float32, copy=True).contiguous(), k)
 
 
 def linear_int8(x, w):

@@ -289,6 +289,20 @@ def test_shared_and_foreign_layers_of_a_model():
         net.d(*[torch.randn(3, 1, 16, device="cuda")] * 3)
 
 
+def test_a_quantised_weight_is_a_copy():
+    """Training on after the quantisation changes neither the codes nor the bias."""
+    from mmearth_train_amd.int8 import linear_int8, quantize_weight
+    layer = torch.nn.Linear(40, 24).cuda()
+    x = torch.randn(5, 40, device="cuda")
+    for bias in (layer.bias, layer.bias.detach()[:1].expand(24)):
+        with torch.no_grad():
+            p = quantize_weight(layer.weight, bias)
+            y = linear_int8(x, p)
+            layer.weight.add_(1.0)
+            layer.bias.add_(1.0)
+            assert torch.equal(y, linear_int8(x, p))
+
+
 def nn_loss(y, t):
     return torch.nn.functional.cross_entropy(y, t)
 
