@@ -139,7 +139,8 @@ __global__ __launch_bounds__(256) void i8_quant_kernel(const T* __restrict__ x, 
                                                        float* __restrict__ scale) {
   __shared__ unsigned red[4];
   const int t = threadIdx.x % TPR;
-  for (int m = blockIdx.x * (256 / TPR) + threadIdx.x / TPR; m < M; m += gridDim.x * (256 / TPR)) {
+  // (unsigned: the step past the last row, at most 2^24 rows on, may pass 31 bits)
+  for (unsigned m = blockIdx.x * (256 / TPR) + threadIdx.x / TPR; m < (unsigned)M; m += gridDim.x * (256 / TPR)) {
     i8_quant_row<T, TPR, NV, RAGGED>(x + (size_t)m * ldx, K, q + (size_t)m * ldq, ldq, scale + m, t, red);
     if (TPR == 256) __syncthreads();      // red is written again
   }
