@@ -47,13 +47,14 @@ def quantize_moments(m, v):
 class _Plan:
     """Device tables and state of one parameter list."""
 
-    def __init__(self, params, groups_of, device, bits, max_norm):
-        self.params, self.device, self.bits = params, device, bits
+    def __init__(self, params, counts, device, bits, max_norm):
+        self.params, self.counts, self.device, self.bits = params, counts, device, bits          # counts: parameters of every group
+        self.shapes = [(p.shape, p.stride()) for p in params]          # the moments lie in this element order, also where a parameter is laid out anew later
         numels = [p.numel() for p in params]
         self.offsets, self.size = moment_layout(numels)
         nt = len(params)
         self.table = np.zeros(nt, _TABLE)
-        self.table["n"], self.table["off"], self.table["group"] = numels, self.offsets, groups_of
+        self.table["n"], self.table["off"], self.table["group"] = numels, self.offsets, np.repeat(np.arange(len(counts)), counts)
         self.table["dt"], self.table["p"] = [_DTYPES[p.dtype] for p in params], [p.data_ptr() for p in params]
         per = -(-self.table["n"] // CHUNK)
         self.chunk_first = np.zeros(nt + 1, np.int32)
@@ -103,6 +104,10 @@ class _Plan:
                 err = call(torch._C._cuda_getCurrentRawStream(self.device.index))
         _lib.check(err, what)
 
+    def views(self, flat):
+        """A flat moment buffer as one tensor per parameter."""
+        return [flat.as_strided(shape, stride, o) for (shape, stride), o in zip(self.shapes, self.offsets)]
+
     def store(self, m, v):
         """The inverse: flat fp32 moments into the state."""
         if self.bits == 32:
@@ -115,10 +120,6 @@ class _Plan:
             km, kv, sm, sv = quantize_moments(m[a:b], v[a:b])
             self.m[a:b], self.v[a:b] = km, kv
             self.ms[a // BLOCK:b // BLOCK], self.vs[a // BLOCK:b // BLOCK] = sm, sv
-
-
-def _view(flat, offset, p):
-    return flat.as_strided(p.shape, p.stride(), offset)       # the moments lie in the parameter's own element order
 
 
 class AdamW(torch.optim.Optimizer):
@@ -174,11 +175,11 @@ class AdamW(torch.optim.Optimizer):
                 if p.device != device:
                     raise ValueError(f"the parameters of one optimizer are on one device: {device} and {p.device}")
             self._check_apart()
-        except ValueError:
+            if self._plan is not None:
+                self._rebuild()
+        except Exception:
             self.param_groups.pop()
             raise
-        if self._plan is not None:
-            self._rebuild()
 
     def _check_apart(self):
         """Two workgroups update two parameters at once: their memory must not overlap."""
@@ -191,15 +192,16 @@ class AdamW(torch.optim.Optimizer):
             raise RuntimeError("run one eager step before capturing one: the state is made on the first")
         _lib.host_tensors()
         params = [p for g in self.param_groups for p in g["params"]]
-        groups_of = [i for i, g in enumerate(self.param_groups) for _ in g["params"]]
         self._check_apart()
-        return _Plan(params, groups_of, params[0].device, self.state_bits, self.max_norm)
+        return _Plan(params, [len(g["params"]) for g in self.param_groups], params[0].device, self.state_bits, self.max_norm)
 
     def _rebuild(self):
         """The state for a longer parameter list, with the moments and step counts of the old one."""
         old, new = self._plan, self._build()
         values = old.values()
         where = {id(p): i for i, p in enumerate(new.params)}
+        if any(new.orders[where[id(p)]] != order for p, order in zip(old.params, old.orders)):
+            raise ValueError("a parameter has another shape or its elements in another order than when the optimizer first ran")
         into = [torch.zeros(new.size, device=new.device) for _ in range(2)]
         for i, p in enumerate(old.params):
             j = where[id(p)]
@@ -213,6 +215,8 @@ class AdamW(torch.optim.Optimizer):
     def plan(self):
         if self._plan is None:
             self._plan = self._build()
+        elif [len(g["params"]) for g in self.param_groups] != self._plan.counts:
+            raise RuntimeError("the groups' parameters are not those of the first step: add_param_group adds some, others take a new optimizer")
         return self._plan
 
     @property
@@ -281,10 +285,9 @@ class AdamW(torch.optim.Optimizer):
         state = {}
         if self._plan is not None:
             plan, steps = self._plan, self._plan.steps.tolist()
-            m, v = plan.values()
-            for i, (p, o) in enumerate(zip(plan.params, plan.offsets)):
+            for i, (m, v) in enumerate(zip(*map(plan.views, plan.values()))):
                 if steps[i]:
-                    state[i] = {"step": torch.tensor(float(steps[i])), "exp_avg": _view(m, o, p).clone(), "exp_avg_sq": _view(v, o, p).clone()}
+                    state[i] = {"step": torch.tensor(float(steps[i])), "exp_avg": m.clone(), "exp_avg_sq": v.clone()}
         return {"state": state, "param_groups": groups}
 
     @torch.no_grad()
@@ -300,14 +303,14 @@ class AdamW(torch.optim.Optimizer):
         plan = self.plan
         ids = [i for g in groups for i in g["params"]]
         entries = [state_dict["state"].get(i) for i in ids]
-        for p, st in zip(plan.params, entries):
-            if st is not None and (st["exp_avg"].shape != p.shape or st["exp_avg_sq"].shape != p.shape):
-                raise ValueError(f"loaded moments of shape {tuple(st['exp_avg'].shape)} for a parameter of shape {tuple(p.shape)}")
+        for (shape, _), st in zip(plan.shapes, entries):
+            if st is not None and (st["exp_avg"].shape != shape or st["exp_avg_sq"].shape != shape):
+                raise ValueError(f"loaded moments of shape {tuple(st['exp_avg'].shape)} for a parameter of shape {tuple(shape)}")
         for mine, g in zip(self.param_groups, groups):
             mine.update({k: v for k, v in g.items() if k in self.defaults or k not in _TORCH_ONLY})
         into = [plan.m, plan.v] if self.state_bits == 32 else [torch.zeros(plan.size, device=plan.device) for _ in range(2)]
         for flat, key in zip(into, ("exp_avg", "exp_avg_sq")):
-            views = [_view(flat, o, p) for p, o in zip(plan.params, plan.offsets)]
+            views = plan.views(flat)
             there = [(view, st[key]) for view, st in zip(views, entries) if st is not None]
             absent = [view for view, st in zip(views, entries) if st is None]
             if there:

@@ -542,3 +542,40 @@ def test_loading_views_of_the_state_itself_and_lists_with_holes(bits):
     opt.load_state_dict(sd | {"state": {0: sd["state"][0]}})
     m, v = opt.flat_moments()
     assert not m[opt.offsets[1]:].any() and not v[opt.offsets[1]:].any() and opt.plan.steps.tolist() == [1, 0, 0]
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_parameter_laid_out_anew_keeps_its_moments_in_place(bits):
+    """Its moments stay in the order of the first step: in a checkpoint, and a list that grows does not take them over misplaced."""
+    from mmearth_train_amd.optim import AdamW
+    w, more = torch.nn.Parameter(torch.randn(6, 4, 3, 3, device="cuda")), torch.nn.Parameter(torch.randn(40, device="cuda"))
+    w.grad = torch.randn_like(w)
+    opt = AdamW([w], state_bits=bits)
+    opt.step()
+    before = opt.state_dict()["state"][0]
+    w.data = w.data.contiguous(memory_format=torch.channels_last)
+    after = opt.state_dict()["state"][0]
+    assert torch.equal(before["exp_avg"], after["exp_avg"]) and torch.equal(before["exp_avg_sq"], after["exp_avg_sq"])
+    with pytest.raises(ValueError, match="another order"):
+        opt.add_param_group({"params": [more]})
+    assert len(opt.param_groups) == 1
+    w.data = w.data.contiguous()
+    opt.add_param_group({"params": [more]})
+    more.grad = torch.ones_like(more)
+    opt.step()
+    assert opt.plan.steps.tolist() == [2, 1]
+
+
+def test_edited_lists_are_refused():
+    from mmearth_train_amd.optim import AdamW
+    a, b = (torch.nn.Parameter(torch.ones(300, device="cuda")) for _ in range(2))
+    a.grad, b.grad = torch.ones_like(a), torch.ones_like(b)
+    opt = AdamW([{"params": [a]}, {"params": []}])
+    opt.step()
+    opt.param_groups[0]["params"].append(b)
+    with pytest.raises(RuntimeError, match="add_param_group"):
+        opt.step()
+    assert torch.equal(b, torch.ones_like(b))
+    opt.param_groups[0]["params"].pop()
+    opt.step()
+    assert opt.plan.steps.tolist() == [2]
