@@ -69,15 +69,17 @@ static void linear_i8(const MpmaeI8Args& a, hipStream_t st) {
            a.ldy, a.M, a.N);
     return;
   }
-  // Tile by the number of tiles that 256 compute units get (us of the product alone; M x K -> N):
+  // Tile by the number of tiles that 256 compute units get (us of the product alone; M x K -> N; the last column with its remainder in pieces):
   //                          32 x 64   64 x 64  128 x 64  128 x 128  256 x 128  256 x 256
-  //   49 x 2816 -> 11264         9.5      10.0      15.6       18.4       31.5       13.9
-  //   784 x 2816 -> 2816        20.4      18.0      19.4       22.0       38.9       28.7
-  //   12544 x 512 -> 2048       47.5      35.2      30.8       33.1       34.6       45.0
-  //   6272 x 2048 -> 2048       60.8      45.5      42.4       38.7       40.5       70.2
-  //   25088 x 640 -> 2560      125.6      84.6      68.8       71.6       63.4       92.0
-  //   4096 x 4096 -> 4096      135.2      96.7      79.3       70.8       72.7       61.3
-  //   12544 x 2048 -> 4096                                    128.8                 118.6
+  //   49 x 2816 -> 11264         9.8      10.1      15.6       17.5       30.4       17.5
+  //   784 x 2816 -> 2816        20.5      17.6      17.9       19.7       34.5       19.5
+  //   12544 x 512 -> 2048       52.5      35.2      29.0       28.8       29.7       31.1
+  //   1568 x 1024 -> 4096       23.1      17.9      17.2       14.7       18.3       14.1
+  //   6272 x 2048 -> 2048       64.2      44.9      39.5       36.3       36.0       35.7
+  //   25088 x 640 -> 2560      132.8      86.3      66.5       61.7       57.8       68.4
+  //   25088 x 160 -> 640        25.5      19.2      15.7       15.5       15.3       20.9
+  //   4096 x 4096 -> 4096      146.3     100.0      76.6       68.7       70.6       58.6
+  //   12544 x 2048 -> 4096     247.2     164.7     124.6      114.1      122.8      102.7
   // 256 x 256 reads LDS least per product, but a workgroup has a compute unit to itself: it needs a long k to cover its first loads and its stores.
   if (count(32, 64) <= 512) return tiles<T, 32, 64, 2, 2, 128, 4>(a, st);
   if (count(64, 64) <= 1024) return tiles<T, 64, 64, 2, 2, 128, 3>(a, st);
