@@ -34,9 +34,11 @@ uint64_t order_of(const at::Tensor& t) {
 }
 
 // gather(params, table, device, out, orders, update) -> (tensors with a gradient, whether a parameter has moved, None or [indices whose gradient lies in another element order])
-// table: address of the host copy of MpmaeAdamwTensor[len(params)], whose parameter addresses are brought up to date; out: address of the gradients'
-// addresses, 0 where there is none; orders: address of one word per parameter, 0 before the first call, that holds it to its element order (its moments lie
-// in the same); update: the parameters with a gradient are about to be written.
+// table: address of the host copy of MpmaeAdamwTensor[len(params)], whose parameter addresses are brought up to date; device: index of the GPU, -1 for host
+// memory; out: address of the gradients' addresses, 0 where there is none; orders: address of one word per parameter, 0 before the first call, that holds it to
+// its element order (its moments lie in the same); update: the parameters with a gradient are about to be written.
+// The whole list is looked over first: a refusal leaves the table, the orders and the parameters' versions as they were, so that the call after it still sees what
+// has moved.
 PyObject* gather(PyObject*, PyObject* args) {
   PyObject* list;
   unsigned long long expected_at, out_at, orders_at;
@@ -48,47 +50,48 @@ PyObject* gather(PyObject*, PyObject* args) {
   PyObject* other = nullptr;
   try {
     const Py_ssize_t count = PyList_GET_SIZE(list);
-    Py_ssize_t grads = 0;
-    bool moved = false;
     for (Py_ssize_t i = 0; i < count; ++i) {
       PyObject* o = PyList_GET_ITEM(list, i);
       const char* wrong = nullptr;
       if (!THPVariable_Check(o)) wrong = "is not a tensor";
       else {
         const at::Tensor& p = THPVariable_Unpack(o);
-        if (p.layout() != at::kStrided || !p.device().is_cuda() || p.device().index() != device) wrong = "has left the optimizer's device";
+        if (p.layout() != at::kStrided || p.device().index() != device || p.device().is_cuda() != (device >= 0)) wrong = "has left the optimizer's device";
         else if (p.numel() != want[i].n || code_of(p.scalar_type()) != want[i].dt) wrong = "has another size or type than when the optimizer first ran";
         else if (!p.is_non_overlapping_and_dense()) wrong = "is not dense in memory";
-        else if (const uint64_t order = order_of(p); orders[i] && orders[i] != order) wrong = "has its elements in another order than when the optimizer first ran";
-        else {
-          orders[i] = order;
-          const at::Tensor& g = p.grad();
-          void* const at = p.data_ptr();
-          moved |= want[i].p != at;
-          want[i].p = at;
-          out[i] = 0;
-          if (g.defined()) {
-            if (g.layout() != at::kStrided) wrong = "has a sparse gradient";
-            else if (g.device() != p.device() || g.scalar_type() != p.scalar_type() || g.sizes() != p.sizes()) wrong = "has a gradient of another device, type or shape";
-            else {
-              ++grads;
-              if (update) p.unsafeGetTensorImpl()->bump_version();      // the kernel writes it behind autograd's back: a stale saved tensor has to be noticed
-              if (same_order(p, g)) out[i] = reinterpret_cast<uint64_t>(g.data_ptr());
-              else {
-                if (!other && !(other = PyList_New(0))) return nullptr;
-                PyObject* k = PyLong_FromSsize_t(i);
-                const int err = k ? PyList_Append(other, k) : -1;
-                Py_XDECREF(k);
-                if (err) { Py_DECREF(other); return nullptr; }
-              }
-            }
-          }
+        else if (orders[i] && orders[i] != order_of(p)) wrong = "has its elements in another order than when the optimizer first ran";
+        else if (const at::Tensor& g = p.grad(); g.defined()) {
+          if (g.layout() != at::kStrided) wrong = "has a sparse gradient";
+          else if (g.device() != p.device() || g.scalar_type() != p.scalar_type() || g.sizes() != p.sizes()) wrong = "has a gradient of another device, type or shape";
+          else (void)g.data_ptr();      // (throws where there is no memory behind it)
         }
+        if (!wrong) (void)p.data_ptr();
       }
-      if (wrong) {
-        Py_XDECREF(other);
-        return PyErr_Format(PyExc_ValueError, "parameter %zd %s", i, wrong);
-      }
+      if (wrong) return PyErr_Format(PyExc_ValueError, "parameter %zd %s", i, wrong);
+    }
+    Py_ssize_t grads = 0;
+    bool moved = false;
+    for (Py_ssize_t i = 0; i < count; ++i) {
+      const at::Tensor& p = THPVariable_Unpack(PyList_GET_ITEM(list, i));
+      const at::Tensor& g = p.grad();
+      out[i] = 0;
+      if (!g.defined()) continue;
+      ++grads;
+      if (same_order(p, g)) { out[i] = reinterpret_cast<uint64_t>(g.data_ptr()); continue; }
+      if (!other && !(other = PyList_New(0))) return nullptr;
+      PyObject* k = PyLong_FromSsize_t(i);
+      const int err = k ? PyList_Append(other, k) : -1;
+      Py_XDECREF(k);
+      if (err) { Py_DECREF(other); return nullptr; }
+    }
+    // nothing fails from here on
+    for (Py_ssize_t i = 0; i < count; ++i) {
+      const at::Tensor& p = THPVariable_Unpack(PyList_GET_ITEM(list, i));
+      void* const at = p.data_ptr();
+      moved |= want[i].p != at;
+      want[i].p = at;
+      orders[i] = order_of(p);
+      if (update && p.grad().defined()) p.unsafeGetTensorImpl()->bump_version();      // the kernel writes it behind autograd's back: a stale saved tensor has to be noticed
     }
     PyObject* const flag = moved ? Py_True : Py_False;
     return other ? Py_BuildValue("nON", grads, flag, other) : Py_BuildValue("nOO", grads, flag, Py_None);

@@ -579,3 +579,24 @@ def test_edited_lists_are_refused():
     opt.param_groups[0]["params"].pop()
     opt.step()
     assert opt.plan.steps.tolist() == [2]
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_refused_step_does_not_lose_what_has_moved(bits):
+    """A parameter moves and a later one's gradient is refused: once that is put right, the step writes the new memory and leaves the old."""
+    from mmearth_train_amd.optim import AdamW
+    params, twin = params_of([300, 5000], DT[:1], 20), params_of([300, 5000], DT[:1], 20)
+    a, b = AdamW(params, state_bits=bits), AdamW(twin, state_bits=bits)
+    for ps in (params, twin):
+        grads_for(ps, 90)
+    a.step(), b.step()
+    old = params[0].data
+    kept = old.clone()
+    params[0].data = old.clone()
+    good = params[1].grad
+    params[1].grad = good.to_sparse()
+    with pytest.raises(ValueError, match="parameter 1 has a sparse"):
+        a.step()
+    params[1].grad = good
+    a.step(), b.step()
+    assert torch.equal(old, kept) and all(torch.equal(p, q) for p, q in zip(params, twin)) and a.plan.steps.tolist() == [2, 2]

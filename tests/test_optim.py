@@ -121,6 +121,46 @@ def test_native_reader_refuses_what_it_cannot_address():
     assert host.gather([], table.ctypes.data, 0, out.ctypes.data, out.ctypes.data, True) == (0, False, None)
 
 
+def _reader_state(params):
+    from mmearth_train_amd import optim
+    table = np.zeros(len(params), optim._TABLE)
+    table["n"], table["p"] = [p.numel() for p in params], [p.data_ptr() for p in params]
+    return table, np.zeros(len(params), np.uint64), np.zeros(len(params), np.uint64)
+
+
+@pytest.mark.parametrize("count,refused", [(2, 1), (2, 0), (1, 0), (3, 2)])
+def test_a_refused_list_does_not_lose_what_has_moved(count, refused):
+    """The native reader over host memory (device -1): parameters move, one gradient is refused, it is put right: the next call still reports the move, and the
+    refusal itself left addresses, orders and versions alone."""
+    from mmearth_train_amd import _lib
+    host = _lib.host_tensors()
+    params = [torch.nn.Parameter(torch.ones(300 + i)) for i in range(count)]
+    for p in params:
+        p.grad = torch.ones_like(p)
+    table, out, orders = _reader_state(params)
+    read = lambda: host.gather(params, table.ctypes.data, -1, out.ctypes.data, orders.ctypes.data, True)  # noqa: E731
+    assert read() == (count, False, None)
+    old = [p.data for p in params]                            # (alive: no new tensor can take their place)
+    for p in params:
+        p.data = p.data.clone()
+    good = params[refused].grad
+    for bad in (torch.ones_like(good).to_sparse(), None):
+        if bad is None:                                       # of another shape, given behind autograd's back
+            params[refused].grad = good
+            params[refused].grad.data = torch.ones(7)
+        else:
+            params[refused].grad = bad
+        keep, versions = (table.copy(), orders.copy()), [p._version for p in params]
+        with pytest.raises(ValueError, match=f"parameter {refused} has a"):
+            read()
+        assert np.array_equal(table, keep[0]) and np.array_equal(orders, keep[1]) and versions == [p._version for p in params]
+    params[refused].grad = torch.ones_like(params[refused])
+    assert read() == (count, True, None)
+    assert table["p"].tolist() == [p.data_ptr() for p in params] and out.tolist() == [p.grad.data_ptr() for p in params]
+    assert not set(table["p"].tolist()) & {p.data_ptr() for p in old}
+    assert read() == (count, False, None)
+
+
 @pytest.fixture(scope="module")
 def lib():
     from mmearth_train_amd import _lib
