@@ -102,6 +102,28 @@ PyObject* gather(PyObject*, PyObject* args) {
   }
 }
 
+// same_lists(param_groups, params, counts) -> whether the groups' lists, one after the other, hold these very parameters, counts[g] of them in group g
+PyObject* same_lists(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  if (nargs != 3 || !PyList_Check(args[0]) || !PyList_Check(args[1]) || !PyList_Check(args[2]))
+    return PyErr_Format(PyExc_TypeError, "same_lists(param_groups, params, counts): three lists");
+  const Py_ssize_t ngroups = PyList_GET_SIZE(args[0]), total = PyList_GET_SIZE(args[1]);
+  if (ngroups != PyList_GET_SIZE(args[2])) Py_RETURN_FALSE;
+  Py_ssize_t at = 0;
+  for (Py_ssize_t g = 0; g < ngroups; ++g) {
+    PyObject* const group = PyList_GET_ITEM(args[0], g);
+    PyObject* const list = PyDict_Check(group) ? PyDict_GetItemString(group, "params") : nullptr;      // (borrowed)
+    if (!list || !PyList_Check(list)) Py_RETURN_FALSE;
+    const Py_ssize_t n = PyList_GET_SIZE(list);
+    const long want = PyLong_AsLong(PyList_GET_ITEM(args[2], g));
+    if (want == -1 && PyErr_Occurred()) return nullptr;
+    if (n != want || at + n > total) Py_RETURN_FALSE;
+    for (Py_ssize_t i = 0; i < n; ++i)
+      if (PyList_GET_ITEM(list, i) != PyList_GET_ITEM(args[1], at + i)) Py_RETURN_FALSE;
+    at += n;
+  }
+  return PyBool_FromLong(at == total);
+}
+
 // linear_i8(x, q, scale, bias or None, k, stream, address of mpmae_linear_i8, of mpmae_linear_i8_part_bytes) -> y. The checks, the output, the workspace and the call
 // of one int8 linear layer: in Python they take 11 us, longer than the kernel for a single row.
 PyObject* linear_i8(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
@@ -159,6 +181,7 @@ PyObject* linear_i8(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
 }
 
 PyMethodDef methods[] = {{"gather", gather, METH_VARARGS, "addresses of parameters and gradients"},
+                         {"same_lists", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(same_lists)), METH_FASTCALL, "whether parameter lists are still the same"},
                          {"linear_i8", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(linear_i8)), METH_FASTCALL, "int8 linear layer"}, {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host_tensors", nullptr, -1, methods};
 

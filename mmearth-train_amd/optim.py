@@ -132,8 +132,9 @@ class AdamW(torch.optim.Optimizer):
 
     Parameters without a gradient are left alone. The update is formed in fp32 and rounded once to the parameter's type. Steps are counted on the
     device: a captured step replays as the next one, with the learning rate it was captured with; run one eager step before the capture.
-    `param_groups` hold lr, betas, eps, weight_decay and may be changed between steps; lr is a number. The moments are in `flat_moments()` and
-    `state_dict()`; `state` stays empty.
+    `param_groups` hold lr, betas, eps, weight_decay and may be changed between steps; lr is a number. Their lists of parameters stay those of the first
+    step, object for object (a call after another edit than `add_param_group` is refused; `model.load_state_dict(assign=True)` puts new parameters into the
+    model, for a new optimizer). The moments are in `flat_moments()` and `state_dict()`; `state` stays empty.
     """
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, *, state_bits=32, max_norm=None):
@@ -157,6 +158,8 @@ class AdamW(torch.optim.Optimizer):
             raise ValueError(f"betas lie in [0, 1): {g['betas']}")
 
     def add_param_group(self, group):
+        if self._plan is not None:
+            self.plan          # (refuses lists that were edited)
         super().add_param_group(group)
         try:
             self._check_group(self.param_groups[-1])
@@ -215,7 +218,7 @@ class AdamW(torch.optim.Optimizer):
     def plan(self):
         if self._plan is None:
             self._plan = self._build()
-        elif [len(g["params"]) for g in self.param_groups] != self._plan.counts:
+        elif not _lib.host_tensors().same_lists(self.param_groups, self._plan.params, self._plan.counts):
             raise RuntimeError("the groups' parameters are not those of the first step: add_param_group adds some, others take a new optimizer")
         return self._plan
 
@@ -250,7 +253,7 @@ class AdamW(torch.optim.Optimizer):
         plan = self.plan
         grads, moved, other = _lib.host_tensors().gather(plan.params, plan.table_at, plan.device.index, plan.grads_at, plan.orders_at, True)
         plan.stale |= moved
-        if plan.stale:                                 # (`p.data = ...`, `model.load_state_dict(assign=True)`)
+        if plan.stale:                                 # (`p.data = ...`)
             if torch.cuda.is_current_stream_capturing():
                 raise RuntimeError("a parameter has moved in memory: run one eager step before capturing one")
             self._check_apart()
@@ -284,7 +287,7 @@ class AdamW(torch.optim.Optimizer):
             at += len(g["params"])
         state = {}
         if self._plan is not None:
-            plan, steps = self._plan, self._plan.steps.tolist()
+            plan, steps = self.plan, self._plan.steps.tolist()
             for i, (m, v) in enumerate(zip(*map(plan.views, plan.values()))):
                 if steps[i]:
                     state[i] = {"step": torch.tensor(float(steps[i])), "exp_avg": m.clone(), "exp_avg_sq": v.clone()}

@@ -600,3 +600,33 @@ def test_a_refused_step_does_not_lose_what_has_moved(bits):
     params[1].grad = good
     a.step(), b.step()
     assert torch.equal(old, kept) and all(torch.equal(p, q) for p, q in zip(params, twin)) and a.plan.steps.tolist() == [2, 2]
+
+
+def test_replaced_and_exchanged_parameters_are_refused():
+    """Lists of the same lengths that hold other parameters: nothing is updated, nothing saved or loaded under a wrong index."""
+    from mmearth_train_amd.optim import AdamW
+    a, b, new = (torch.nn.Parameter(torch.ones(300, device="cuda")) for _ in range(3))
+    for p in (a, b, new):
+        p.grad = torch.ones_like(p)
+    opt = AdamW([{"params": [a], "lr": 1e-3}, {"params": [b], "lr": 1e-1}])
+    opt.step()
+    keep = [p.detach().clone() for p in (a, b, new)]
+    one, two = opt.param_groups
+    saved = opt.state_dict()
+
+    def put(x, y):
+        one["params"][0], two["params"][0] = x, y
+
+    for x, y in ((new, b), (b, a)):
+        put(x, y)
+        for call in (opt.step, opt.state_dict, opt.flat_moments, lambda: opt.load_state_dict(saved), lambda: opt.add_param_group({"params": [new]})):
+            with pytest.raises(RuntimeError, match="add_param_group"):
+                call()
+        assert all(torch.equal(p, q) for p, q in zip((a, b, new), keep)) and len(opt.param_groups) == 2
+    put(a, b)
+    opt.param_groups.reverse()
+    with pytest.raises(RuntimeError, match="add_param_group"):
+        opt.step()
+    opt.param_groups.reverse()
+    opt.step()
+    assert opt.plan.steps.tolist() == [2, 2]

@@ -161,6 +161,20 @@ def test_a_refused_list_does_not_lose_what_has_moved(count, refused):
     assert read() == (count, False, None)
 
 
+def test_lists_are_compared_object_for_object():
+    from mmearth_train_amd import _lib
+    same = _lib.host_tensors().same_lists
+    a, b, c = (torch.nn.Parameter(torch.zeros(3)) for _ in range(3))
+    group = lambda *ps: {"params": list(ps), "lr": 1.0}  # noqa: E731
+    assert same([group(a, b), group(c)], [a, b, c], [2, 1]) and same([], [], []) and same([group(), group(a)], [a], [0, 1])
+    for groups in ([group(a, b), group(b)], [group(b, a), group(c)], [group(a, c), group(b)], [group(a), group(b, c)], [group(c), group(a, b)], [group(a, b)],
+                   [group(a, b), group(c), group()], [group(a, b), group()], [group(a, b), {"params": (c,)}], [group(a, b), 3]):
+        assert not same(groups, [a, b, c], [2, 1])
+    assert not same([group(a)], [a, b], [1]) and not same([group(a, b)], [a], [2])
+    with pytest.raises(TypeError):
+        same([], [], 3)
+
+
 @pytest.fixture(scope="module")
 def lib():
     from mmearth_train_amd import _lib
