@@ -372,7 +372,7 @@ int mpmae_gemm_mx(int epi, const MpmaeGemmArgs* args, const uint32_t* scales_a, 
 
 /* ---- 8-bit integer linear layer (inference of nn.Linear: pwconv1 / pwconv2 / head of the dense network, convnextv2.py:46-52) ----------------
  * mpmae_quant_i8: M rows of K elements (dt: 0 fp32, 1 bf16, 2 fp16; ldx elements from row to row) to int8 codes q[M][ldq] and scale[M]:
- *   scale = max|x| / 127, q = round(127 x / max|x|), half to even; a row with NaN or infinity: scale NaN, codes 0. ldq: a multiple of 128, zeros from K on.
+ *   scale = max|x| / 127, q = round(127 x / max|x|), half to even; a row with NaN or infinity: scale NaN, codes 0. ldq: K rounded up to a multiple of 128, zeros from K on.
  * mpmae_linear_i8: y[M][N] = sx[m] sw[n] (q w^T)[m][n] + bias[n] (bias may be NULL, fp32), y in x's type: quantises the rows of x into the workspace
  *   q[M][ldq], sx[M] and multiplies them with w[N][ldw] (from mpmae_quant_i8; ldw == ldq); exact 32-bit integer sums (K <= 131071). q, w, part 16-byte
  *   aligned. part: workspace of mpmae_linear_i8_part_bytes(M, N, K) bytes for products whose k is split (NULL where that is 0). */

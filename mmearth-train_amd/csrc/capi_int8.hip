@@ -96,8 +96,10 @@ static void linear_i8(const MpmaeI8Args& a, hipStream_t st) {
   if (a.K >= 1024) return tiles<T, 128, 128, 2, 2, 128, 2>(a, st);
   tiles<T, 128, 64, 2, 2, 128, 2>(a, st);
 }
+// (ldq: K rounded up and nothing else, since the split of k, and with it the workspace, goes by K alone and rows of fewer than eight elements pad one I8_KPAD)
+static int row_bytes(int K) { return (K + I8_KPAD - 1) / I8_KPAD * I8_KPAD; }
 static bool bad_rows(int dt, const void* x, long long ldx, int M, int K, const void* q, int ldq, const float* scale) {
-  return dt < 0 || dt > 2 || !x || !q || !scale || M < 1 || K < 1 || K > 131071 || ldx < 0 || ldq < K || ldq % I8_KPAD || ((uintptr_t)q & 15);
+  return dt < 0 || dt > 2 || !x || !q || !scale || M < 1 || K < 1 || K > 131071 || ldx < 0 || ldq != row_bytes(K) || ((uintptr_t)q & 15);
 }
 
 extern "C" {
@@ -111,8 +113,8 @@ int mpmae_quant_i8(int dt, const void* x, long long ldx, int M, int K, int8_t* q
 }
 
 long long mpmae_linear_i8_part_bytes(int M, int N, int K) {
-  if (M < 1 || N < 1 || K < 1) return 0;
-  const int s = i8_splits(M, N, (K + I8_KPAD - 1) / I8_KPAD * I8_KPAD);
+  if (M < 1 || N < 1 || K < 1 || K > 131071) return 0;
+  const int s = i8_splits(M, N, row_bytes(K));
   return s > 1 ? (long long)s * M * N * 4 : 0;
 }
 

@@ -146,10 +146,10 @@ PyObject* linear_i8(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     const auto plain = [&](const at::Tensor& t, at::ScalarType type, int64_t numel) {
       return t.device() == q.device() && t.scalar_type() == type && t.is_contiguous() && t.numel() == numel;
     };
-    if (q.dim() != 2 || q.scalar_type() != at::kChar || !q.is_contiguous() || q.size(0) < 1 || q.size(1) % 128 || q.size(1) < k || k < 1 ||
+    if (q.dim() != 2 || q.scalar_type() != at::kChar || !q.is_contiguous() || q.size(0) < 1 || k < 1 || q.size(1) != (k + 127) / 128 * 128 ||
         !plain(scale, at::kFloat, q.size(0)) || (args[3] != Py_None && !plain(THPVariable_Unpack(args[3]), at::kFloat, q.size(0))) ||
         (reinterpret_cast<uintptr_t>(q.data_ptr()) & 15))
-      return PyErr_Format(PyExc_ValueError, "a weight is what quantize_weight makes: int8 rows of a multiple of 128, fp32 scales and bias, contiguous");
+      return PyErr_Format(PyExc_ValueError, "a weight is what quantize_weight makes: int8 rows of K rounded up to a multiple of 128, fp32 scales and bias, contiguous");
     const int64_t n = q.size(0), kp = q.size(1);
     at::DimVector shape(x.sizes().begin(), x.sizes().end());
     shape.back() = n;

@@ -216,6 +216,17 @@ def test_refusals_on_the_device():
             linear_int8(torch.zeros(2, 16, device="cuda"), bad)
 
 
+def test_wider_rows_of_codes_are_refused():
+    """Codes padded further than K rounded up: refused on the host, before anything is launched."""
+    from mmearth_train_amd.int8 import Int8Weight, linear_int8, quantize_weight
+    for k, wide, m in ((3900, 4096, 64), (7, 256, 3), (100, 384, 20)):
+        p = quantize_weight(torch.ones(5, k, device="cuda"))
+        q = torch.zeros(5, wide, device="cuda", dtype=torch.int8)
+        q[:, :p.q.shape[1]] = p.q
+        with pytest.raises(ValueError, match="quantize_weight makes"):
+            linear_int8(torch.ones(m, k, device="cuda"), Int8Weight(q, p.scale, None, k))
+
+
 def test_a_network_is_trained_with_8_bit_moments_and_served_in_int8(tmp_path):
     """The dense network as a user has it: fine-tuned by the 8-bit AdamW, then quantised, saved, loaded and served."""
     from mmearth_train_amd import convnextv2

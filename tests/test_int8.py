@@ -36,6 +36,23 @@ def test_library_refuses_bad_arguments():
     assert lib.mpmae_linear_i8(0, None, None) != 0
 
 
+def test_rows_of_codes_are_k_rounded_up_and_no_longer():
+    """Wider rows would split k in more parts than the workspace was sized for (64 x 3900 -> 1000: none by K, four by rows of 4096 bytes) and leave the padding of
+    rows of fewer than eight elements unwritten. hipErrorInvalidValue is 1; a call that is let through fails here for want of a GPU, with another error."""
+    from mmearth_train_amd import _lib
+    lib = _lib.load()
+    room = C.create_string_buffer(4096)
+    at = (C.addressof(room) + 15) & ~15
+    assert lib.mpmae_linear_i8_part_bytes(64, 1000, 3900) == 0 and lib.mpmae_linear_i8_part_bytes(64, 1000, 4096) == 4 * 4 * 64 * 1000
+    for k, wide in ((3900, 4096), (3900, 3968 + 128), (1, 256), (7, 256), (128, 256), (129, 384), (100, 0), (100, -128)):
+        assert lib.mpmae_quant_i8(0, at, k, 1, k, at, wide, at, None) == 1, (k, wide)
+        args = _lib.I8Args(x=at, q=at, sx=at, w=at, sw=at, bias=None, y=at, part=at, ldx=k, ldy=1000, M=64, N=1000, K=k, ldq=wide, ldw=wide)
+        assert lib.mpmae_linear_i8(0, C.byref(args), None) == 1, (k, wide)
+    # (products whose workspace is missing are refused, whatever their size)
+    args = _lib.I8Args(x=at, q=at, sx=at, w=at, sw=at, bias=None, y=at, part=None, ldx=4096, ldy=1000, M=64, N=1000, K=4096, ldq=4096, ldw=4096)
+    assert lib.mpmae_linear_i8(0, C.byref(args), None) == 1
+
+
 def test_struct_matches_the_header(tmp_path):
     from mmearth_train_amd import _lib
     src = tmp_path / "s.c"
