@@ -586,7 +586,7 @@ int mpmae_sumsq(const float* x, size_t n, float* out, mpmae_stream_t stream);
  * call), fp32 / bf16 / fp16 parameters and gradients mixed freely, moments in fp32 (bits = 32) or in 8 bits (bits = 8). Per element, with
  * coef = min(1, max_norm / (|g| + 1e-6)) over the gradients of ALL tensors (max_norm <= 0: no norm, coef = 1):
  *   m = b1 m + (1 - b1) coef g;  v = b2 v + (1 - b2) (coef g)^2;  p = p (1 - lr wd) - lr / (1 - b1^t) m / (sqrt(v) / sqrt(1 - b2^t) + eps)
- * A tensor without a gradient (NULL) is left alone and its step count stands; so does everything when the norm is not finite (norm_skip[1] = 1).
+ * A tensor without a gradient (NULL) is left alone and its step count stands; so does everything when the norm, in fp32, is not finite (norm_skip[1] = 1).
  * Steps are counted on the device, so a captured call replays as the next step.
  *   - grads (HOST): gradient address of every tensor, passed to the kernels by value; in the parameter's own dense element order;
  *   - groups (HOST): {lr, beta1, beta2, eps, weight_decay} of every parameter group;

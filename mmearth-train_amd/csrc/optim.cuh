@@ -128,7 +128,7 @@ __global__ __launch_bounds__(512) void adamw_hyper_kernel(AdamwGroups groups, co
     double s = 0.0;
     for (int i = threadIdx.x; i < npartials; i += 512) s += partials[i];
     const double norm = sqrt(adamw_block_sum(s, red));
-    const bool bad = !(norm < (double)INFINITY);
+    const bool bad = !((float)norm < INFINITY);      // (as the norm is reported: one past fp32's range reads as infinity)
     if (threadIdx.x == 0) { norm_skip[0] = (float)norm; norm_skip[1] = bad ? 1.f : 0.f; }
     if (bad) return;
     coef = (float)fmin(1.0, max_norm / (norm + 1e-6));
@@ -157,7 +157,8 @@ template <typename T, bool FULL>
 __device__ __forceinline__ void adamw32_chunk(T* __restrict__ p, const T* __restrict__ g, float* __restrict__ m, float* __restrict__ v, long long n,
                                               long long base, const AdamwHyper& h) {
 #pragma clang fp contract(off)      // (the same bits whichever form a chunk takes)
-  const float b1 = (float)h.b1, c1 = (float)(h.c1 * h.coef), b2 = (float)h.b2, c2 = (float)(h.c2 * h.coef * h.coef);
+  // (the clip factor meets the gradient first: its square alone leaves fp32's range at norms whose clipped gradients are ordinary numbers)
+  const float b1 = (float)h.b1, c1 = (float)h.c1, b2 = (float)h.b2, c2 = (float)h.c2, coef = (float)h.coef;
   const long long i = base + threadIdx.x * 8;
   if (!FULL && i >= n) return;
   float pv[8], gv[8], mv[8], vv[8];
@@ -167,8 +168,9 @@ __device__ __forceinline__ void adamw32_chunk(T* __restrict__ p, const T* __rest
   ld8(v + i, vv);
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
-    mv[e] = __builtin_fmaf(b1, mv[e], c1 * gv[e]);
-    vv[e] = __builtin_fmaf(b2, vv[e], c2 * gv[e] * gv[e]);
+    const float gc = gv[e] * coef;
+    mv[e] = __builtin_fmaf(b1, mv[e], c1 * gc);
+    vv[e] = __builtin_fmaf(b2, vv[e], c2 * gc * gc);
     pv[e] = __builtin_fmaf(pv[e], h.decay, -(h.step * mv[e] / __builtin_fmaf(sqrtf(vv[e]), h.isbc2, h.eps)));
   }
   adamw_st8<T, FULL>(p, i, n, pv);

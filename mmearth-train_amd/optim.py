@@ -127,7 +127,7 @@ class AdamW(torch.optim.Optimizer):
 
     state_bits   32: fp32 moments. 8: both moments in one byte per element and one fp32 scale per 256 elements.
     max_norm     not None: the gradients enter the update scaled by min(1, max_norm / (norm + 1e-6)), norm over all of them as in
-                 torch.nn.utils.clip_grad_norm_ (the gradients themselves stay as they are); `grad_norm` is that norm on the device. A step whose
+                 torch.nn.utils.clip_grad_norm_ (the gradients themselves stay as they are); `grad_norm` is that norm, fp32, on the device. A step whose
                  norm is not finite changes nothing (`skipped` is then 1), as the fused pretraining step does.
 
     Parameters without a gradient are left alone. The update is formed in fp32 and rounded once to the parameter's type. Steps are counted on the

@@ -630,3 +630,40 @@ def test_replaced_and_exchanged_parameters_are_refused():
     opt.param_groups.reverse()
     opt.step()
     assert opt.plan.steps.tolist() == [2, 2]
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("size", [1e18, 1e20, 1e22, 1e30, 1e34])
+@pytest.mark.parametrize("types", [DT[:1], DT[1:2]], ids=["fp32", "bf16"])
+def test_clip_of_large_finite_norms(bits, size, types):
+    """coef * g is an ordinary number, coef^2 and g^2 are not: the moments take the clipped gradient's square, on the first step and after."""
+    from mmearth_train_amd.optim import AdamW
+    params = params_of([257, 4100], types, 21)
+    refs = [Ref(p, bits) for p in params]
+    opt = AdamW(params, lr=1e-3, state_bits=bits, max_norm=1.0)
+    for k in range(2):
+        grads_for(params, 110 + k, scale=size)
+        norm = math.sqrt(sum(float(p.grad.double().square().sum()) for p in params))
+        coef = float(np.float32(min(1.0, 1.0 / (norm + 1e-6))))
+        opt.step()
+        assert float(opt.skipped) == 0.0 and abs(float(opt.grad_norm) - norm) <= 2 * U * norm
+        for p, r in zip(params, refs):
+            r.step(p.grad, coef, 1e-3, 0.9, 0.999, 1e-8, 1e-2)
+    check(opt, params, refs, bits)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_norm_past_the_range_of_fp32_skips_the_step(bits):
+    """Every element finite, the norm not a number of fp32: `grad_norm` reads infinity, `skipped` 1, and nothing has changed."""
+    from mmearth_train_amd.optim import AdamW
+    params = params_of([300, 5000], DT[:2], 22)
+    opt = AdamW(params, state_bits=bits, max_norm=1.0)
+    grads_for(params, 1)
+    opt.step()
+    keep = [p.detach().clone() for p in params], [x.clone() for x in opt.flat_moments()], opt.plan.steps.clone()
+    for p in params:
+        p.grad.fill_(1e37)                                     # 5300 of them: a norm of 7.3e38
+    opt.step()
+    assert float(opt.skipped) == 1.0 and float(opt.grad_norm) == float("inf")
+    assert all(torch.equal(a, b.detach()) for a, b in zip(keep[0], params))
+    assert all(torch.equal(a, b) for a, b in zip(keep[1], opt.flat_moments())) and torch.equal(keep[2], opt.plan.steps)
