@@ -82,6 +82,7 @@ class _Plan:
                                    hyper=at(self.hyper), partials=at(self.partials), norm_skip=at(self.norm_skip), m=at(self.m), v=at(self.v),
                                    ms=at(self.ms), vs=at(self.vs), max_norm=float(max_norm or 0.0), nt=nt, npartials=npart, bits=bits)
         self.ref, self.stale = C.byref(self.args), False          # stale: parameters have moved and the device table does not know
+        self.captured = False                                     # a graph holds the addresses of these buffers
         self.table_at, self.grads_at, self.orders_at = self.table.ctypes.data, self.grads.ctypes.data, self.orders.ctypes.data
         _lib.host_tensors().gather(params, self.table_at, device.index, self.grads_at, self.orders_at, False)      # (holds them to the order that offsets go by)
         torch.cuda.current_stream(device).synchronize()      # the tables and zeroed moments are there for whatever stream steps first
@@ -97,11 +98,11 @@ class _Plan:
 
     def launch(self, what, call):
         """call(stream) with this plan's device as the current one."""
-        if torch._C._cuda_getDevice() == self.device.index:
-            err = call(torch._C._cuda_getCurrentRawStream(self.device.index))
-        else:
+        if torch._C._cuda_getDevice() != self.device.index:
             with torch.cuda.device(self.device):
-                err = call(torch._C._cuda_getCurrentRawStream(self.device.index))
+                return self.launch(what, call)
+        self.captured |= torch.cuda.is_current_stream_capturing()
+        err = call(torch._C._cuda_getCurrentRawStream(self.device.index))
         _lib.check(err, what)
 
     def views(self, flat):
@@ -131,7 +132,8 @@ class AdamW(torch.optim.Optimizer):
                  norm is not finite changes nothing (`skipped` is then 1), as the fused pretraining step does.
 
     Parameters without a gradient are left alone. The update is formed in fp32 and rounded once to the parameter's type. Steps are counted on the
-    device: a captured step replays as the next one, with the learning rate it was captured with; run one eager step before the capture.
+    device: a captured step replays as the next one, with the learning rate it was captured with; run one eager step before the capture. The graph
+    holds the addresses of the optimizer's buffers: the optimizer has to outlive it, and takes no further groups after a capture.
     `param_groups` hold lr, betas, eps, weight_decay and may be changed between steps; lr is a number. Their lists of parameters stay those of the first
     step, object for object (a call after another edit than `add_param_group` is refused; `model.load_state_dict(assign=True)` puts new parameters into the
     model, for a new optimizer). The moments are in `flat_moments()` and `state_dict()`; `state` stays empty.
@@ -158,8 +160,8 @@ class AdamW(torch.optim.Optimizer):
             raise ValueError(f"betas lie in [0, 1): {g['betas']}")
 
     def add_param_group(self, group):
-        if self._plan is not None:
-            self.plan          # (refuses lists that were edited)
+        if self._plan is not None and self.plan.captured:
+            raise RuntimeError("a captured step of this optimizer holds its buffers, which a longer parameter list replaces: add groups before the capture")
         super().add_param_group(group)
         try:
             self._check_group(self.param_groups[-1])
@@ -260,6 +262,7 @@ class AdamW(torch.optim.Optimizer):
             plan.d_table.copy_(torch.from_numpy(plan.table.view(np.uint8)))
             plan.stale = False
         if not grads:
+            plan.captured |= torch.cuda.is_current_stream_capturing()
             plan.norm_skip.zero_()
             return loss
         copies = []                                    # gradients in another element order than their parameter's, alive until the launches are queued

@@ -667,3 +667,30 @@ def test_a_norm_past_the_range_of_fp32_skips_the_step(bits):
     assert float(opt.skipped) == 1.0 and float(opt.grad_norm) == float("inf")
     assert all(torch.equal(a, b.detach()) for a, b in zip(keep[0], params))
     assert all(torch.equal(a, b) for a, b in zip(keep[1], opt.flat_moments())) and torch.equal(keep[2], opt.plan.steps)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_no_group_is_added_behind_a_captured_step(bits):
+    """A longer list takes new buffers; a graph would go on writing the old, freed ones. The refusal leaves optimizer and graph as they were."""
+    from mmearth_train_amd.optim import AdamW
+    params, twin = params_of([700, 300, 40], DT[:1], 23), params_of([700, 300, 40], DT[:1], 23)
+    a, b = AdamW(params[:2], state_bits=bits), AdamW(twin[:2], state_bits=bits)
+    for ps in (params, twin):
+        grads_for(ps, 120)
+    a.step(), b.step()
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        a.step()
+    with pytest.raises(RuntimeError, match="captured"):
+        a.add_param_group({"params": [params[2]]})
+    assert len(a.param_groups) == 1
+    for _ in range(2):
+        graph.replay()
+        b.step()
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(params, twin))
+        assert all(torch.equal(x, y) for x, y in zip(a.flat_moments(), b.flat_moments()))
+    b.add_param_group({"params": [twin[2]]})                   # (nothing was captured here)
+    b.step()
+    assert b.plan.steps.tolist() == [4, 4, 1]
