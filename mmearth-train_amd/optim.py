@@ -214,6 +214,7 @@ class AdamW(torch.optim.Optimizer):
                 a[new.offsets[j]:new.offsets[j] + p.numel()] = b[old.offsets[i]:old.offsets[i] + p.numel()]
             new.steps[j] = old.steps[i]
         new.store(*into)
+        torch.cuda.current_stream(new.device).synchronize()      # the old buffers go back to the stream that made them, which may be another one
         self._plan = new
 
     @property

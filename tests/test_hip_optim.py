@@ -694,3 +694,22 @@ def test_no_group_is_added_behind_a_captured_step(bits):
     b.add_param_group({"params": [twin[2]]})                   # (nothing was captured here)
     b.step()
     assert b.plan.steps.tolist() == [4, 4, 1]
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_group_added_on_another_stream(bits):
+    """The old state is read on that stream and freed on the first one's: the reads are done when the call returns, and the values are the ones they were."""
+    from mmearth_train_amd.optim import AdamW
+    params = params_of([5_000_000, 300], DT[:1], 24)
+    opt = AdamW(params[:1], state_bits=bits)
+    grads_for(params, 130)
+    opt.step()
+    m, v = (x.clone() for x in opt.flat_moments())
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        opt.add_param_group({"params": params[1:]})
+        assert s.query()
+    fill = [torch.full_like(x, 7.0) for x in (m, v) for _ in range(2)]
+    assert all(torch.equal(x[:5_000_000], y[:5_000_000]) for x, y in zip((m, v), opt.flat_moments())) and len(fill) == 4
+    assert opt.plan.steps.tolist() == [1, 0]
