@@ -337,11 +337,13 @@ def host_tensors():
     if _host is None:
         import importlib.machinery
         import importlib.util
-        load()
+        lib = load()
         path = os.path.join(_HERE, "_host_tensors.so")
         if not os.path.isfile(path):
             raise HipLibraryError(f"{path} not found: build it with `python -c 'import __graft_entry__ as g; g.build()'`")
         loader = importlib.machinery.ExtensionFileLoader("_host_tensors", path)
-        _host = importlib.util.module_from_spec(importlib.util.spec_from_loader("_host_tensors", loader))
-        loader.exec_module(_host)
+        host = importlib.util.module_from_spec(importlib.util.spec_from_loader("_host_tensors", loader))
+        loader.exec_module(host)
+        host.bind(*(C.cast(f, c_void_p).value for f in (lib.mpmae_linear_i8, lib.mpmae_linear_i8_part_bytes, lib.mpmae_quant_i8)))
+        _host = host
     return _host

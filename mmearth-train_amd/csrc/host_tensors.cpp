@@ -1,15 +1,23 @@
-// Host side of the many-tensor operators: reads the addresses of a parameter list and of its gradients straight from the tensors.
+// Host side of the many-tensor operators and of the int8 layer.
 //
-// A Python loop over `p.data_ptr(), p.grad, p.grad.data_ptr()` and the checks costs ~0.6 us per tensor; for the 144 tensors of the smallest
+// The former read the addresses of a parameter list and of its gradients straight from the tensors: a Python loop over `p.data_ptr(), p.grad, p.grad.data_ptr()` and the checks costs ~0.6 us per tensor; for the 144 tensors of the smallest
 // network that is several times the kernel's own run time.
+#include <ATen/core/LegacyTypeDispatch.h>
 #include <ATen/core/Tensor.h>
+#include <ATen/core/dispatch/Dispatcher.h>
 #include <ATen/core/grad_mode.h>
 #include <ATen/ops/empty.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPStream.h>
+#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/library.h>
 #include <Python.h>
 #include <cstdint>
 #include <exception>
+#include <optional>
+#include <tuple>
 #include "../../include/mpmae_hip.h"
 
 namespace {
@@ -124,65 +132,148 @@ PyObject* same_lists(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   return PyBool_FromLong(at == total);
 }
 
-// linear_i8(x, q, scale, bias or None, k, stream, address of mpmae_linear_i8, of mpmae_linear_i8_part_bytes) -> y. The checks, the output, the workspace and the call
-// of one int8 linear layer: in Python they take 11 us, longer than the kernel for a single row.
-PyObject* linear_i8(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
-  if (nargs != 8 || !THPVariable_Check(args[0]) || !THPVariable_Check(args[1]) || !THPVariable_Check(args[2]) || (args[3] != Py_None && !THPVariable_Check(args[3])))
-    return PyErr_Format(PyExc_TypeError, "linear_i8(x, q, scale, bias, k, stream, entry, part_bytes)");
-  const long long k = PyLong_AsLongLong(args[4]);
-  void* const stream = PyLong_AsVoidPtr(args[5]);
-  const auto entry = reinterpret_cast<int (*)(int, const MpmaeI8Args*, mpmae_stream_t)>(PyLong_AsVoidPtr(args[6]));
-  const auto part_bytes = reinterpret_cast<long long (*)(int, int, int)>(PyLong_AsVoidPtr(args[7]));
-  if (PyErr_Occurred()) return nullptr;
-  try {
-    at::Tensor x = THPVariable_Unpack(args[0]);
-    const at::Tensor &q = THPVariable_Unpack(args[1]), &scale = THPVariable_Unpack(args[2]);
-    if (x.requires_grad() && at::GradMode::is_enabled()) return PyErr_Format(PyExc_RuntimeError, "linear_int8 has no backward pass: call it under torch.no_grad()");
-    const int dt = code_of(x.scalar_type());
-    if (dt < 0 || x.layout() != at::kStrided) return PyErr_Format(PyExc_ValueError, "inputs are dense fp32, bf16 or fp16 tensors, not %s", c10::toString(x.scalar_type()));
-    if (x.dim() < 1 || x.size(-1) != k) return PyErr_Format(PyExc_ValueError, "inputs end in %lld elements, the weight's", k);
-    if (x.device() != q.device() || !x.device().is_cuda())
-      return PyErr_Format(PyExc_ValueError, "the input is on %s, the weight on %s", x.device().str().c_str(), q.device().str().c_str());
-    const auto plain = [&](const at::Tensor& t, at::ScalarType type, int64_t numel) {
-      return t.device() == q.device() && t.scalar_type() == type && t.is_contiguous() && t.numel() == numel;
-    };
-    if (q.dim() != 2 || q.scalar_type() != at::kChar || !q.is_contiguous() || q.size(0) < 1 || k < 1 || q.size(1) != (k + 127) / 128 * 128 ||
-        !plain(scale, at::kFloat, q.size(0)) || (args[3] != Py_None && !plain(THPVariable_Unpack(args[3]), at::kFloat, q.size(0))) ||
-        (reinterpret_cast<uintptr_t>(q.data_ptr()) & 15))
-      return PyErr_Format(PyExc_ValueError, "a weight is what quantize_weight makes: int8 rows of K rounded up to a multiple of 128, fp32 scales and bias, contiguous");
-    const int64_t n = q.size(0), kp = q.size(1);
-    at::DimVector shape(x.sizes().begin(), x.sizes().end());
-    shape.back() = n;
-    c10::OptionalDeviceGuard guard(x.device());
-    at::Tensor y = at::empty(shape, x.options().requires_grad(false));
-    if (y.numel()) {
-      if (x.dim() != 2 || (x.stride(1) != 1 && k > 1)) {
-        x = x.reshape({-1, k});
-        if (x.stride(1) != 1 && k > 1) x = x.contiguous();
-      }
-      const int64_t m = x.size(0);
-      if (m > INT32_MAX || n > INT32_MAX) return PyErr_Format(PyExc_ValueError, "more than 2^31 - 1 rows");
-      const int64_t codes = m * (kp + 4), part_at = (codes + 15) / 16 * 16;
-      const at::Tensor ws = at::empty({part_at + part_bytes((int)m, (int)n, (int)k)}, x.options().dtype(at::kByte).requires_grad(false));
-      char* at = static_cast<char*>(ws.data_ptr());
-      MpmaeI8Args a{};
-      a.x = x.data_ptr(); a.q = reinterpret_cast<int8_t*>(at); a.sx = reinterpret_cast<float*>(at + m * kp);
-      a.w = static_cast<const int8_t*>(q.data_ptr()); a.sw = static_cast<const float*>(scale.data_ptr());
-      a.bias = args[3] == Py_None ? nullptr : static_cast<const float*>(THPVariable_Unpack(args[3]).data_ptr());
-      a.y = y.data_ptr(); a.part = reinterpret_cast<int*>(at + part_at);
-      a.ldx = x.stride(0); a.ldy = n; a.M = (int)m; a.N = (int)n; a.K = (int)k; a.ldq = (int)kp; a.ldw = (int)kp;
-      if (const int err = entry(dt, &a, stream)) return PyErr_Format(PyExc_RuntimeError, "linear_i8 failed with hipError %d", err);
-    }
-    return THPVariable_Wrap(std::move(y));
-  } catch (const std::exception& e) {
-    PyErr_SetString(PyExc_RuntimeError, e.what());
-    return nullptr;
-  }
+// ---- the int8 linear layer and its quantiser, as operators of torch's dispatcher (mpmae::linear_int8, mpmae::quantize_int8): a trace, a dispatch mode or a
+// functional transform sees the call. What they allocate is filled by this library, behind the dispatcher's back, so nothing above may take it for the result.
+using LinearEntry = int (*)(int, const MpmaeI8Args*, mpmae_stream_t);
+using PartBytes = long long (*)(int, int, int);
+using QuantEntry = int (*)(int, const void*, long long, int, int, int8_t*, int, float*, mpmae_stream_t);
+LinearEntry linear_entry = nullptr;          // of libmpmae_hip.so, from bind()
+PartBytes part_bytes = nullptr;
+QuantEntry quant_entry = nullptr;
+
+PyObject* bind(PyObject*, PyObject* args) {
+  unsigned long long linear, part, quant;
+  if (!PyArg_ParseTuple(args, "KKK", &linear, &part, &quant)) return nullptr;
+  linear_entry = reinterpret_cast<LinearEntry>(linear);
+  part_bytes = reinterpret_cast<PartBytes>(part);
+  quant_entry = reinterpret_cast<QuantEntry>(quant);
+  Py_RETURN_NONE;
 }
+
+// rows of k elements that lie next to each other
+at::Tensor rows_of(const at::Tensor& x, int64_t k) {
+  if (x.dim() == 2 && (x.stride(1) == 1 || k == 1)) return x;
+  const at::Tensor r = x.reshape({-1, k});
+  return r.stride(1) == 1 || k == 1 ? r : r.contiguous();
+}
+mpmae_stream_t stream_of(const at::Tensor& t) { return c10::hip::getCurrentHIPStream(t.device().index()).stream(); }
+constexpr int64_t row_bytes(int64_t k) { return (k + 127) / 128 * 128; }
+
+std::tuple<at::Tensor, at::Tensor> quantize_gpu(const at::Tensor& w) {
+  const int dt = code_of(w.scalar_type());
+  TORCH_CHECK_VALUE(w.dim() == 2 && w.numel() > 0 && w.size(1) <= 131071 && w.size(0) <= INT32_MAX && dt >= 0 && w.layout() == at::kStrided,
+                    "a weight is a dense matrix [N, K] of fp32, bf16 or fp16, K at most 131071");
+  TORCH_CHECK_VALUE(w.device().is_cuda(), "this layer runs on the GPU only: the weight is on ", w.device());
+  TORCH_CHECK(quant_entry, "the kernels are not loaded: mmearth_train_amd.int8.load_ops()");
+  const int64_t n = w.size(0), k = w.size(1);
+  c10::OptionalDeviceGuard guard(w.device());
+  const at::Tensor r = rows_of(w, k);
+  at::Tensor q = at::empty({n, row_bytes(k)}, w.options().dtype(at::kChar)), scale = at::empty({n}, w.options().dtype(at::kFloat));
+  const int err = quant_entry(dt, r.data_ptr(), r.stride(0), (int)n, (int)k, static_cast<int8_t*>(q.data_ptr()), (int)q.size(1), static_cast<float*>(scale.data_ptr()), stream_of(w));
+  TORCH_CHECK(!err, "quant_i8 failed with hipError ", err);
+  return {q, scale};
+}
+
+std::tuple<at::Tensor, at::Tensor> quantize_meta(const at::Tensor& w) {
+  TORCH_CHECK_VALUE(w.dim() == 2, "a weight is a matrix [N, K]");
+  const c10::SymInt n = w.sym_size(0), kp = (w.sym_size(1) + 127) / 128 * 128;
+  return {at::empty_symint({n, kp}, w.options().dtype(at::kChar)), at::empty_symint({n}, w.options().dtype(at::kFloat))};
+}
+
+// y = x W^T + bias: checks, output, workspace and launch (in Python they take 11 us, longer than the kernel for a single row)
+at::Tensor linear_gpu(const at::Tensor& x, const at::Tensor& q, const at::Tensor& scale, const std::optional<at::Tensor>& bias, int64_t k) {
+  const int dt = code_of(x.scalar_type());
+  TORCH_CHECK_VALUE(dt >= 0 && x.layout() == at::kStrided, "inputs are dense fp32, bf16 or fp16 tensors, not ", x.scalar_type());
+  TORCH_CHECK_VALUE(x.dim() >= 1 && x.size(-1) == k, "inputs end in ", k, " elements, the weight's");
+  TORCH_CHECK_VALUE(x.device() == q.device() && x.device().is_cuda(), "the input is on ", x.device(), ", the weight on ", q.device());
+  const auto plain = [&](const at::Tensor& t, at::ScalarType type, int64_t numel) {
+    return t.device() == q.device() && t.scalar_type() == type && t.is_contiguous() && t.numel() == numel;
+  };
+  TORCH_CHECK_VALUE(q.dim() == 2 && q.scalar_type() == at::kChar && q.is_contiguous() && q.size(0) >= 1 && k >= 1 && q.size(1) == row_bytes(k) &&
+                        plain(scale, at::kFloat, q.size(0)) && (!bias || plain(*bias, at::kFloat, q.size(0))) && !(reinterpret_cast<uintptr_t>(q.data_ptr()) & 15),
+                    "a weight is what quantize_weight makes: int8 rows of K rounded up to a multiple of 128, fp32 scales and bias, contiguous");
+  TORCH_CHECK(linear_entry, "the kernels are not loaded: mmearth_train_amd.int8.load_ops()");
+  const int64_t n = q.size(0), kp = q.size(1);
+  at::DimVector shape(x.sizes().begin(), x.sizes().end());
+  shape.back() = n;
+  c10::OptionalDeviceGuard guard(x.device());
+  at::Tensor y = at::empty(shape, x.options());
+  if (!y.numel()) return y;
+  const at::Tensor r = rows_of(x, k);
+  const int64_t m = r.size(0);
+  TORCH_CHECK_VALUE(m <= INT32_MAX && n <= INT32_MAX, "more than 2^31 - 1 rows");
+  const int64_t codes = m * (kp + 4), part_at = (codes + 15) / 16 * 16;
+  const at::Tensor ws = at::empty({part_at + part_bytes((int)m, (int)n, (int)k)}, x.options().dtype(at::kByte));
+  char* at = static_cast<char*>(ws.data_ptr());
+  MpmaeI8Args a{};
+  a.x = r.data_ptr(); a.q = reinterpret_cast<int8_t*>(at); a.sx = reinterpret_cast<float*>(at + m * kp);
+  a.w = static_cast<const int8_t*>(q.data_ptr()); a.sw = static_cast<const float*>(scale.data_ptr());
+  a.bias = bias ? static_cast<const float*>(bias->data_ptr()) : nullptr;
+  a.y = y.data_ptr(); a.part = reinterpret_cast<int*>(at + part_at);
+  a.ldx = r.stride(0); a.ldy = n; a.M = (int)m; a.N = (int)n; a.K = (int)k; a.ldq = (int)kp; a.ldw = (int)kp;
+  const int err = linear_entry(dt, &a, stream_of(x));
+  TORCH_CHECK(!err, "linear_i8 failed with hipError ", err);
+  return y;
+}
+
+at::Tensor linear_meta(const at::Tensor& x, const at::Tensor& q, const at::Tensor&, const std::optional<at::Tensor>&, int64_t k) {
+  TORCH_CHECK_VALUE(x.dim() >= 1 && x.sym_size(-1) == k, "inputs end in ", k, " elements, the weight's");
+  c10::SymDimVector shape(x.sym_sizes().begin(), x.sym_sizes().end());
+  shape.back() = q.sym_size(0);
+  return at::empty_symint(shape, x.options());
+}
+
+using Linear = at::Tensor(const at::Tensor&, const at::Tensor&, const at::Tensor&, const std::optional<at::Tensor>&, int64_t);
+at::Tensor call_linear(const at::Tensor& x, const at::Tensor& q, const at::Tensor& scale, const std::optional<at::Tensor>& bias, int64_t k) {
+  static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow("mpmae::linear_int8", "").typed<Linear>();
+  return op.call(x, q, scale, bias, k);
+}
+
+// no backward pass and no tangent: an input that needs either is refused
+at::Tensor linear_autograd(const at::Tensor& x, const at::Tensor& q, const at::Tensor& scale, const std::optional<at::Tensor>& bias, int64_t k) {
+  const bool forward = c10::AutogradState::get_tls_state().get_fw_grad_mode();
+  for (const at::Tensor* t : {&x, &scale, bias ? &*bias : &x}) {
+    TORCH_CHECK(!(t->requires_grad() && at::GradMode::is_enabled()), "linear_int8 has no backward pass: call it under torch.no_grad()");
+    TORCH_CHECK(!(forward && t->_fw_grad(0).defined()), "linear_int8 has no derivative: an input is a dual tensor of forward-mode differentiation");
+  }
+  at::AutoDispatchBelowADInplaceOrView below;
+  return call_linear(x, q, scale, bias, k);
+}
+
+// linear_i8(x, q, scale, bias or None, k) -> y
+PyObject* linear_i8(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  if (nargs != 5 || !THPVariable_Check(args[0]) || !THPVariable_Check(args[1]) || !THPVariable_Check(args[2]) || (args[3] != Py_None && !THPVariable_Check(args[3])))
+    return PyErr_Format(PyExc_TypeError, "linear_i8(x, q, scale, bias, k)");
+  const long long k = PyLong_AsLongLong(args[4]);
+  if (PyErr_Occurred()) return nullptr;
+  return THPVariable_Wrap(call_linear(THPVariable_Unpack(args[0]), THPVariable_Unpack(args[1]), THPVariable_Unpack(args[2]),
+                                      args[3] == Py_None ? std::optional<at::Tensor>() : std::optional<at::Tensor>(THPVariable_Unpack(args[3])), k));
+  END_HANDLE_TH_ERRORS
+}
+
+TORCH_LIBRARY(mpmae, m) {
+  m.def("linear_int8(Tensor x, Tensor q, Tensor scale, Tensor? bias, int k) -> Tensor");
+  m.def("quantize_int8(Tensor weight) -> (Tensor, Tensor)");
+}
+TORCH_LIBRARY_IMPL(mpmae, CUDA, m) {
+  m.impl("linear_int8", linear_gpu);
+  m.impl("quantize_int8", quantize_gpu);
+}
+TORCH_LIBRARY_IMPL(mpmae, CPU, m) {      // (their refusals)
+  m.impl("linear_int8", linear_gpu);
+  m.impl("quantize_int8", quantize_gpu);
+}
+TORCH_LIBRARY_IMPL(mpmae, Meta, m) {
+  m.impl("linear_int8", linear_meta);
+  m.impl("quantize_int8", quantize_meta);
+}
+TORCH_LIBRARY_IMPL(mpmae, Autograd, m) { m.impl("linear_int8", linear_autograd); }
 
 PyMethodDef methods[] = {{"gather", gather, METH_VARARGS, "addresses of parameters and gradients"},
                          {"same_lists", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(same_lists)), METH_FASTCALL, "whether parameter lists are still the same"},
-                         {"linear_i8", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(linear_i8)), METH_FASTCALL, "int8 linear layer"}, {nullptr, nullptr, 0, nullptr}};
+                         {"linear_i8", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(linear_i8)), METH_FASTCALL, "int8 linear layer"},
+                         {"bind", bind, METH_VARARGS, "entry points of the kernel library"}, {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host_tensors", nullptr, -1, methods};
 
 }  // namespace

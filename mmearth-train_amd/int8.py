@@ -7,10 +7,9 @@ channel, activations per row (token, pixel) inside the call, exact integer sums 
 
     x_q = round(127 x / max|x|), s_x = max|x| / 127 per row;  y = s_x s_w (x_q w_q^T) + bias
 
-Inference only: an input that requires a gradient is refused. There is no CPU form.
+Inference only: an input that requires a gradient or carries a tangent is refused. The call is an operator of torch's dispatcher, so traces and exported graphs
+hold it; `load_ops()` before loading one. There is no CPU form.
 """
-import ctypes as C
-
 import torch
 import torch.nn as nn
 
@@ -29,18 +28,15 @@ def _rows(x, k):
     return x, x.shape[0], x.stride(0)
 
 
-def _stream(device):
-    return torch.cuda.current_stream(device).cuda_stream
+_linear = None          # native call, from the first use on
 
 
-_native = None          # (native call, address of mpmae_linear_i8, of mpmae_linear_i8_part_bytes), from the first call on
-
-
-def _load_native():
-    global _native
-    lib, host = _lib.load(), _lib.host_tensors()
-    _native = (host.linear_i8, *(C.cast(f, C.c_void_p).value for f in (lib.mpmae_linear_i8, lib.mpmae_linear_i8_part_bytes)))
-    return _native
+def load_ops():
+    """Registers the operators that a traced or exported network calls (`torch.ops.mpmae.linear_int8`): before `torch.jit.load` of one. `linear_int8` does it by
+    itself."""
+    global _linear
+    _linear = _lib.host_tensors().linear_i8
+    return _linear
 
 
 class Int8Weight:
@@ -68,23 +64,16 @@ def quantize_weight(weight, bias=None):
         raise ValueError(f"a bias is a floating vector [{weight.shape[0]}] on the weight's device")
     if weight.device.type != "cuda":
         raise ValueError(f"this layer runs on the GPU only: the weight is on {weight.device}")
-    n, k = weight.shape
-    w, _, ld = _rows(weight, k)
-    kp = -(-k // _lib.I8_KPAD) * _lib.I8_KPAD
-    q = torch.empty(n, kp, dtype=torch.int8, device=weight.device)
-    scale = torch.empty(n, dtype=torch.float32, device=weight.device)
-    with torch.cuda.device(weight.device):
-        err = _lib.load().mpmae_quant_i8(_DTYPES[w.dtype], w.data_ptr(), ld, n, k, q.data_ptr(), kp, scale.data_ptr(), _stream(weight.device))
-    _lib.check(err, "quant_i8")
+    load_ops()
+    k = int(weight.shape[1])
+    q, scale = torch.ops.mpmae.quantize_int8(_rows(weight.detach(), k)[0])
     # (a copy of the bias too: the codes are those of this moment)
     return Int8Weight(q, scale, None if bias is None else bias.detach().to(torch.float32, copy=True).contiguous(), k)
 
 
 def linear_int8(x, w):
     """y = x W^T + bias for x [..., K] fp32 / bf16 / fp16 on the weight's GPU; y has x's type. A row that holds NaN or infinity gives a row of NaN."""
-    call, entry, part = _native or _load_native()
-    stream = torch._C._cuda_getCurrentRawStream(w.device.index) if w.device.type == "cuda" else 0
-    return call(x, w.q, w.scale, w.bias, w.k, stream, entry, part)          # checks, output, workspace and launch: csrc/host_tensors.cpp
+    return (_linear or load_ops())(x, w.q, w.scale, w.bias, w.k)          # torch.ops.mpmae.linear_int8 with less on the way: csrc/host_tensors.cpp
 
 
 class Int8Linear(nn.Module):

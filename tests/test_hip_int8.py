@@ -325,3 +325,43 @@ def test_hub_serves_in_int8():
     assert isinstance(net.head, Int8Linear) and isinstance(net.stages[0][0].pwconv1, Int8Linear) and net.head.q.is_cuda
     with torch.no_grad():
         assert net(torch.randn(1, 12, 56, 56, device="cuda")).shape == (1, 7)
+
+
+def test_traced_and_exported_layers_compute(tmp_path):
+    """The operator is in the graph, with other inputs and row counts than the traced ones, from a file, and next to the eager call bit for bit."""
+    import warnings
+    from torch.fx.experimental.proxy_tensor import make_fx
+    from mmearth_train_amd.int8 import linear_int8, quantize_model, quantize_weight
+    torch.manual_seed(0)
+    net = quantize_model(torch.nn.Sequential(torch.nn.Linear(96, 200), torch.nn.GELU(), torch.nn.Linear(200, 33)).cuda())
+    xs = [torch.randn(n, 96, device="cuda") for n in (5, 1, 300)]
+    w = torch.randn(40, 96, device="cuda")
+    with torch.no_grad(), warnings.catch_warnings():
+        warnings.simplefilter("error", torch.jit.TracerWarning)
+        want = [net(x) for x in xs]
+        traced = torch.jit.trace(net, xs[0])
+        assert str(traced.inlined_graph).count("mpmae::linear_int8") == 2
+        traced.save(str(tmp_path / "net.pt"))
+        loaded = torch.jit.load(str(tmp_path / "net.pt"))
+        fx = make_fx(net)(xs[0])
+        exported = torch.export.export(net, (xs[0],), strict=False).module()
+        for f, count in ((traced, 3), (loaded, 3), (fx, 1), (exported, 1)):
+            for _ in range(3):
+                for x, y in list(zip(xs, want))[:count]:
+                    junk = torch.full_like(y, 5.0)              # (what an output that nothing writes would hold)
+                    del junk
+                    assert torch.equal(f(x), y)
+        warnings.simplefilter("ignore")                         # (the quantiser's checks of sizes in Python hold for the traced ones)
+        both = torch.jit.trace(lambda x, w: linear_int8(x, quantize_weight(w)), (xs[0], w))
+        assert "mpmae::quantize_int8" in str(both.graph) and "aten::empty" not in str(both.graph)
+        for _ in range(2):
+            assert torch.equal(both(xs[2], 2 * w), linear_int8(xs[2], quantize_weight(2 * w)))
+        # rows under vmap are the rows of the whole call
+        p = quantize_weight(w)
+        assert torch.equal(torch.vmap(lambda x: linear_int8(x, p))(xs[2].view(10, 30, 96)), linear_int8(xs[2], p).view(10, 30, 40))
+        s = torch.cuda.Stream()
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            y = traced(xs[2])
+        torch.cuda.current_stream().wait_stream(s)
+        assert torch.equal(y, want[2])

@@ -93,3 +93,43 @@ def test_a_cpu_input_is_refused_and_modules_copy():
         m(torch.zeros(2, 100))
     for other in (copy.deepcopy(m), pickle.loads(pickle.dumps(m))):
         assert other.q.data_ptr() != m.q.data_ptr() and (other._weight is None or other._weight.q is other.q)
+
+
+def test_the_call_is_an_operator_that_tracing_sees():
+    """On tensors without memory: shapes come out of the operator's own rule, and a graph holds the operator instead of the empty tensor that it fills."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    from torch.fx.experimental.proxy_tensor import make_fx
+    from mmearth_train_amd.int8 import Int8Linear, Int8Weight, linear_int8, load_ops
+    load_ops()
+    m = Int8Linear(100, 7, device="meta")
+    with torch.no_grad():
+        y = m(torch.zeros(2, 3, 100, device="meta", dtype=torch.float16))
+    assert y.shape == (2, 3, 7) and y.dtype == torch.float16 and y.is_meta
+    with pytest.raises(ValueError, match="end in 100"):
+        m(torch.zeros(2, 99, device="meta"))
+    q, scale = torch.ops.mpmae.quantize_int8(torch.zeros(7, 100, device="meta"))
+    assert q.shape == (7, 128) and q.dtype == torch.int8 and scale.shape == (7,) and scale.dtype == torch.float32
+    with FakeTensorMode():
+        for device in ("meta", "cuda"):
+            new = lambda *shape, dtype=torch.float32: torch.empty(*shape, dtype=dtype, device=device)  # noqa: E731, B023
+            w = Int8Weight(new(7, 128, dtype=torch.int8), new(7), new(7), 100)
+            graph = make_fx(lambda x: linear_int8(x, w) * 2)(new(5, 100)).graph  # noqa: B023
+            called = [n.target for n in graph.nodes if n.op == "call_function"]
+            assert torch.ops.mpmae.linear_int8.default in called and not any("empty" in str(t) for t in called), called
+
+
+def test_derivatives_are_refused_not_dropped():
+    import torch.autograd.forward_ad as fwad
+    from mmearth_train_amd.int8 import Int8Linear
+    m, x = Int8Linear(100, 7), torch.ones(2, 100)
+    with pytest.raises(RuntimeError, match="no backward"):
+        m(x.clone().requires_grad_())
+    with fwad.dual_level():
+        with pytest.raises(RuntimeError, match="no derivative"):
+            m(fwad.make_dual(x, torch.ones_like(x)))
+    with pytest.raises(RuntimeError, match="no derivative"):
+        torch.func.jvp(m, (x,), (x,))
+    with pytest.raises(RuntimeError, match="no backward"):
+        torch.func.grad(lambda x: m(x).sum())(x)
+    with pytest.raises(ValueError, match="is on cpu"):          # (without either, the device is what is wrong here)
+        m(x)
