@@ -93,6 +93,9 @@ class Int8Linear(nn.Module):
         w = quantize_weight(linear.weight, linear.bias)
         self = cls(linear.in_features, linear.out_features, linear.bias is not None, device="meta")
         self.q, self.scale, self.bias = w.q, w.scale, w.bias
+        self.training = linear.training
+        for name in _FORWARD_HOOKS:          # (the dictionaries themselves: handles of `register_forward_hook` go on removing from them)
+            setattr(self, name, getattr(linear, name))
         return self
 
     def _apply(self, fn, recurse=True):
@@ -112,14 +115,23 @@ class Int8Linear(nn.Module):
         return f"in_features={self.in_features}, out_features={self.out_features}, bias={self.bias is not None}"
 
 
+_FORWARD_HOOKS = ("_forward_hooks", "_forward_hooks_with_kwargs", "_forward_hooks_always_called", "_forward_pre_hooks", "_forward_pre_hooks_with_kwargs")
+
+
+def _plain(module):
+    """Whether a module is an nn.Linear and nothing more: no subclass (its users may read the weight), no weight that a hook computes (weight norm, pruning), no
+    forward of its own."""
+    return type(module) is nn.Linear and module._parameters.get("weight") is not None and "forward" not in module.__dict__
+
+
 def quantize_model(model, _made=None):
-    """Every nn.Linear of the module tree (on the GPU; no subclasses, whose users may read the weight) becomes an Int8Linear, in place; one that is used in
-    several places stays one. Returns the model."""
+    """Every plain nn.Linear of the module tree (on the GPU) becomes an Int8Linear, in place, and takes its forward hooks along; one that is used in several
+    places stays one, others stay as they are. Returns the model."""
     made = {} if _made is None else _made
     if id(model) in made:
         return made[id(model)]
     made[id(model)] = model
-    if type(model) is nn.Linear:
+    if _plain(model):
         made[id(model)] = Int8Linear.from_linear(model)
         return made[id(model)]
     for name, child in model._modules.items():

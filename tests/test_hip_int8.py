@@ -365,3 +365,31 @@ def test_traced_and_exported_layers_compute(tmp_path):
             y = traced(xs[2])
         torch.cuda.current_stream().wait_stream(s)
         assert torch.equal(y, want[2])
+
+
+def test_quantised_layers_keep_their_hooks():
+    """Forward hooks and pre-hooks run on the new layer as on the old one, and their handles remove them; layers whose weight a hook computes or whose forward was
+    replaced stay as they are."""
+    import torch.nn.utils.prune as prune
+    from mmearth_train_amd.int8 import Int8Linear, quantize_model
+    torch.manual_seed(1)
+    net = torch.nn.Sequential(*[torch.nn.Linear(16, 16) for _ in range(5)]).cuda().eval()
+    seen = []
+    pre = net[0].register_forward_pre_hook(lambda m, a: (seen.append("pre"), (a[0] * 2,))[1])
+    post = net[0].register_forward_hook(lambda m, a, kw, y: (seen.append(type(m)), y + 1)[1], with_kwargs=True)
+    prune.random_unstructured(net[1], "weight", 0.5)
+    net[2] = torch.nn.utils.spectral_norm(net[2])
+    was = net[3].forward
+    net[3].forward = lambda x: was(x) - 1
+    net[3].register_forward_hook(lambda m, a, y: -y)
+    x = torch.randn(4, 16, device="cuda")
+    with torch.no_grad():
+        quantize_model(net)
+        assert [isinstance(m, Int8Linear) for m in net] == [True, False, False, False, True] and not net[0].training
+        y = net[0](x)
+        assert seen == ["pre", Int8Linear]
+        post.remove()
+        assert torch.equal(net[0](x) + 1, y) and seen == ["pre", Int8Linear, "pre"]
+        pre.remove()
+        assert torch.equal(net[0](2 * x) + 1, y) and len(seen) == 3
+        net(x)
