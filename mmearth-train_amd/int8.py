@@ -124,17 +124,12 @@ def _plain(module):
     return type(module) is nn.Linear and module._parameters.get("weight") is not None and "forward" not in module.__dict__
 
 
-def quantize_model(model, _made=None):
+def quantize_model(model):
     """Every plain nn.Linear of the module tree (on the GPU) becomes an Int8Linear, in place, and takes its forward hooks along; one that is used in several
-    places stays one, others stay as they are. Returns the model."""
-    made = {} if _made is None else _made
-    if id(model) in made:
-        return made[id(model)]
-    made[id(model)] = model
-    if _plain(model):
-        made[id(model)] = Int8Linear.from_linear(model)
-        return made[id(model)]
-    for name, child in model._modules.items():
-        if child is not None:
-            model._modules[name] = quantize_model(child, made)
-    return model
+    places stays one, others stay as they are. Returns the model. Nothing is replaced unless every layer can be."""
+    made = {m: Int8Linear.from_linear(m) for m in model.modules() if _plain(m)}
+    for parent in list(model.modules()):
+        for name, child in parent._modules.items():
+            if child in made:
+                parent._modules[name] = made[child]
+    return made.get(model, model)

@@ -393,3 +393,14 @@ def test_quantised_layers_keep_their_hooks():
         pre.remove()
         assert torch.equal(net[0](2 * x) + 1, y) and len(seen) == 3
         net(x)
+
+
+def test_a_refused_layer_leaves_the_model_as_it_was():
+    from mmearth_train_amd.int8 import Int8Linear, quantize_model
+    net = torch.nn.Sequential(torch.nn.Linear(16, 16), torch.nn.Sequential(torch.nn.Linear(16, 8)), torch.nn.Linear(8, 4).double()).cuda()
+    with pytest.raises(ValueError, match="fp32, bf16 or fp16"):
+        quantize_model(net)
+    assert not any(isinstance(m, Int8Linear) for m in net.modules())
+    net[2].float()
+    assert [isinstance(m, Int8Linear) for m in (quantize_model(net)[0], net[1][0], net[2])] == [True] * 3
+    assert isinstance(quantize_model(torch.nn.Linear(4, 4).cuda()), Int8Linear)
