@@ -39,12 +39,13 @@ __device__ __forceinline__ void i8_end8(int i, int K, const Raw8<T>& raw, const 
 // Eight codes. Adding 1.5 * 2^23 rounds x * (127 / a) to the nearest whole number (half to even) and leaves it, as a byte of two's complement, in the low
 // bits of the sum. The rounded factor makes the product wrong by at most 127 * 2^-24 = 7.6e-6, so a code is certain unless the product lies within 2e-5 of a
 // half; those (|x| = a / 2 is a common one in 16-bit types) are decided on the remainder 127 x - r a, which is exact: in fp32 for types of at most 11
-// significant bits, in fp64 for fp32. up: 1, or 2^100 for a row whose reciprocal would overflow; a and inv are those of the row times up.
+// significant bits, in fp64 for fp32. up: 1, or 2^100 for a row whose reciprocal would overflow, 2^-100 where 127 a would; a and inv are those of the row times
+// up (exact for every element that has a code but 0).
 struct I8Row { float a, inv, up; };
 __device__ __forceinline__ I8Row i8_row(unsigned mx) {
   I8Row r;
   r.a = __uint_as_float(mx);
-  r.up = r.a < 1e-30f ? 0x1p100f : 1.f;
+  r.up = r.a < 1e-30f ? 0x1p100f : r.a > 1e30f ? 0x1p-100f : 1.f;
   r.a *= r.up;
   r.inv = 127.f / r.a;
   return r;

@@ -404,3 +404,24 @@ def test_a_refused_layer_leaves_the_model_as_it_was():
     net[2].float()
     assert [isinstance(m, Int8Linear) for m in (quantize_model(net)[0], net[1][0], net[2])] == [True] * 3
     assert isinstance(quantize_model(torch.nn.Linear(4, 4).cuda()), Int8Linear)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("k", [7, 130, 1000, 9000, 20000])
+def test_codes_of_rows_near_the_largest_number(dtype, k):
+    """Rows whose maximum times 127 is no number of fp32, among them exact ties (63.5: half the maximum) and the type's
+    lowest value."""
+    from mmearth_train_amd.int8 import quantize_weight
+    t = DT[dtype]
+    x, _, _ = data(6, k, 1, t, False, 2)
+    x = (x.float() / x.float().abs().amax(1, keepdim=True) * torch.tensor([3.3e38, 1e38, 2.7e36, 2.6e36, 1e31, 1e30], device="cuda")[:, None]).to(t)
+    x[0, 0] = torch.finfo(t).min
+    for r in range(6):
+        a = float(x[r].abs().amax())
+        x[r, 1:k:5] = a / 2                                   # 63.5 -> 64
+        x[r, 2:k:5] = -a / 2
+        if dtype == "fp32" or r:
+            x[r, -1] = (2.0 ** math.floor(math.log2(a)))      # a power of two near the top
+    w = quantize_weight(x)
+    q, s = ref_codes(x)
+    assert torch.equal(w.q[:, :k].cpu().double(), q) and torch.equal(w.scale.cpu().double(), s)
