@@ -51,6 +51,8 @@ __device__ __forceinline__ I8Row i8_row(unsigned mx) {
   return r;
 }
 __device__ __forceinline__ float i8_scale(unsigned mx) { return mx >= 0x7f800000u ? NAN : __uint_as_float(mx) / 127.f; }
+// An output. The sum meets the weight's scale first: with a row near the type's largest number (its lowest value as a mask) sum * sx alone would pass fp32's range.
+__device__ __forceinline__ float i8_out(int sum, float sx, float sw, float bias) { return (float)sum * sw * sx + bias; }
 template <typename T>
 __device__ __forceinline__ uint2 i8_codes(const float (&x)[8], const I8Row& row) {
   constexpr float MAGIC = 12582912.f;
@@ -274,7 +276,7 @@ __global__ __launch_bounds__(512) void i8_skinny_kernel(const T* __restrict__ x,
 #pragma unroll
     for (int v = 0; v < 8; ++v) sum += red[v * MT * NT * 256 + o];
     const int tile = o >> 8, m = (tile / NT) * 16 + ((o >> 4) & 15), n = n0 + (tile % NT) * 16 + (o & 15);
-    if (m < M && n < N) elem_st(y + (size_t)m * ldy + n, (float)sum * (FUSED ? ssx[m] : sa[m]) * sb[n] + (bias ? bias[n] : 0.f));
+    if (m < M && n < N) elem_st(y + (size_t)m * ldy + n, i8_out(sum, FUSED ? ssx[m] : sa[m], sb[n], bias ? bias[n] : 0.f));
   }
 }
 
@@ -455,7 +457,7 @@ __global__ __launch_bounds__(WM * WN * 64, i8_waves_per_simd(i8_tile_lds(BM, BN,
       const float sr = ep[row - m0];
       float v[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = (float)acc[i][2 * jp + (e >> 2)][e & 3] * sr * s[e] + c[e];
+      for (int e = 0; e < 8; ++e) v[e] = i8_out(acc[i][2 * jp + (e >> 2)][e & 3], sr, s[e], c[e]);
       T* out = y + (size_t)row * ldy + col;
       if (past && col + 8 <= N) vec8_st<T, true>(out, v);
       else if (col + 8 <= N) vec8_st(out, v);
@@ -476,6 +478,6 @@ __global__ __launch_bounds__(256) void i8_join_kernel(const int* __restrict__ pa
     int sum = 0;
     for (int s = 0; s < splits; ++s) sum += part[(size_t)s * all + o];
     const int m = (int)(o / N), n = (int)(o - (long long)m * N);
-    elem_st(y + (size_t)m * ldy + n, (float)sum * sa[m] * sb[n] + (bias ? bias[n] : 0.f));
+    elem_st(y + (size_t)m * ldy + n, i8_out(sum, sa[m], sb[n], bias ? bias[n] : 0.f));
   }
 }

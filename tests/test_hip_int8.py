@@ -425,3 +425,18 @@ def test_codes_of_rows_near_the_largest_number(dtype, k):
     w = quantize_weight(x)
     q, s = ref_codes(x)
     assert torch.equal(w.q[:, :k].cpu().double(), q) and torch.equal(w.scale.cpu().double(), s)
+
+
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("m,k,n", [(1, 130, 40), (6, 1000, 33), (8, 3080, 40), (12, 640, 100), (40, 640, 100), (40, 4096, 100), (700, 130, 600)])
+def test_outputs_of_rows_that_hold_the_lowest_value(m, k, n, dtype):
+    """Every form of the product: outputs that are numbers of the type come out as such, also where the scale of x times the integer sum is none."""
+    from mmearth_train_amd.int8 import linear_int8, quantize_weight
+    t = DT[dtype]
+    x, w, b = data(m, k, n, t, True, 12)
+    x[:, ::3] = torch.finfo(t).min
+    x[m - 1] = torch.finfo(t).max / 3
+    w = w / (k if dtype == "fp16" else 64 * k)                # (sums of k products stay below the largest number)
+    y = linear_int8(x, quantize_weight(w, b))
+    assert bool(torch.isfinite(y).all())
+    check(x, w, b, y)
