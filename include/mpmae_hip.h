@@ -658,8 +658,8 @@ int mpmae_program_run(MpmaeProgram* p, int first, int count, mpmae_stream_t main
 /* Hardware queues. ROCm maps HIP streams onto GPU_MAX_HW_QUEUES (default 4) hardware queues, balancing by stream count; streams that
  * share a queue are serialised. A side lane that lands on the main stream's queue costs the whole overlap of the backward (measured
  * 5.4 instead of 4.4 ms per step, and which streams collide depends on how many streams torch / RCCL created earlier). run() therefore
- * PROBES its side lanes at the first replay against a given main stream (two 30 us spin kernels started together: ~50 us when the
- * streams are concurrent, ~80 us on a shared queue) and replaces a colliding lane by a freshly created stream - one host
+ * PROBES its side lanes at the first replay against a given main stream (a kernel on the main stream waits, at most 300 us, for a word that
+ * a kernel behind it on the lane sets, which on a shared queue starts too late) and replaces a colliding lane by a freshly created stream - one host
  * synchronisation, once per (program, main stream). mpmae_program_stream_overlaps() applies the same probe to a stream OUTSIDE the
  * program (gradient-exchange stream, input-stage stream) against the main stream and every side lane: 1 = concurrent with all of them,
  * 0 = shares a queue with one (the caller creates another stream and asks again), < 0 = -(hipError). p == NULL: against the main stream

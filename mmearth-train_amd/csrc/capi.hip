@@ -1043,34 +1043,40 @@ int mpmae_program_stream_wait(MpmaeProgram* p, int signal, mpmae_stream_t stream
 // same queue are serialised. Whether the weight-gradient lane overlaps with the main lane therefore depended on how many streams
 // torch / RCCL had created before the program: measured 4.38 ms per step when the lanes sat on different queues and 5.38 ms when a
 // one-rank RCCL communicator had shifted the side lane onto the main stream's queue (kernel trace: both lanes on queue 4). At the
-// first replay against a given main stream every side lane is therefore PROBED - two 30 us spin kernels, one per stream, started
-// together: concurrent streams finish in ~30 us, a shared queue in ~60 - and a lane that does not overlap is replaced by a freshly
-// created stream (the next queue in the rotation), up to eight times. One host synchronisation, once per (program, main stream).
-__global__ void lane_probe_spin_kernel(unsigned long long ticks) {
+// first replay against a given main stream every side lane is therefore PROBED - a kernel on the main stream waits, at most 300 us, for a word
+// that a kernel launched behind it on the lane sets: on a shared queue the second one starts when the first has ended - and a lane that does not
+// overlap is replaced by a freshly created stream (the next queue in the rotation), up to eight times. One host synchronisation, once per
+// (program, main stream). (Comparing the time of two spin kernels with that of one told streams apart by 30 us; the waits between streams alone
+// vary by as much on some machines, and a stream with a queue of its own was refused one time in five.)
+__global__ void lane_probe_wait_kernel(unsigned* words, unsigned long long ticks) {
   const unsigned long long t0 = __builtin_amdgcn_s_memrealtime();       // 100 MHz
-  while (__builtin_amdgcn_s_memrealtime() - t0 < ticks) __builtin_amdgcn_s_sleep(8);
+  unsigned seen = 0;
+  while (!(seen = __hip_atomic_load(words, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM)) && __builtin_amdgcn_s_memrealtime() - t0 < ticks) __builtin_amdgcn_s_sleep(8);
+  __hip_atomic_store(words + 1, seen, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
 }
+__global__ void lane_probe_set_kernel(unsigned* words) { __hip_atomic_store(words, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM); }
 
-// elapsed time (us) of one spin on `main` [+ one on `side`, started together]; < 0 on any runtime error
-static float lane_probe_us(hipStream_t main, hipStream_t side, hipEvent_t e0, hipEvent_t e1, hipEvent_t es) {
-  const unsigned long long ticks = 3000;                                // 30 us
-  if (hipStreamSynchronize(main) != hipSuccess || (side && hipStreamSynchronize(side) != hipSuccess)) return -1.f;
-  if (hipEventRecord(e0, main) != hipSuccess || (side && hipStreamWaitEvent(side, e0, 0) != hipSuccess)) return -1.f;
-  hipLaunchKernelGGL(lane_probe_spin_kernel, dim3(1), dim3(64), 0, main, ticks);
-  if (side) {
-    hipLaunchKernelGGL(lane_probe_spin_kernel, dim3(1), dim3(64), 0, side, ticks);
-    if (hipEventRecord(es, side) != hipSuccess || hipStreamWaitEvent(main, es, 0) != hipSuccess) return -1.f;
+struct LaneProbe {
+  unsigned* words = nullptr;                                            // pinned host memory: {set by the lane, seen by the main stream}
+  LaneProbe() { if (hipHostMalloc((void**)&words, 2 * sizeof(unsigned), hipHostMallocDefault) != hipSuccess) { words = nullptr; (void)hipGetLastError(); } }
+  ~LaneProbe() { if (words) (void)hipHostFree(words); }
+  LaneProbe(const LaneProbe&) = delete;
+  LaneProbe& operator=(const LaneProbe&) = delete;
+  // 1 both ran at once, 0 one after the other, -1 a runtime error
+  int once(hipStream_t main, hipStream_t side) {
+    hipLaunchKernelGGL(lane_probe_set_kernel, dim3(1), dim3(1), 0, side, words);      // (the first launch on a stream creates its queue)
+    hipLaunchKernelGGL(lane_probe_set_kernel, dim3(1), dim3(1), 0, main, words);
+    if (hipStreamSynchronize(side) != hipSuccess || hipStreamSynchronize(main) != hipSuccess) return -1;
+    volatile unsigned* w = words;
+    w[0] = w[1] = 0;
+    hipLaunchKernelGGL(lane_probe_wait_kernel, dim3(1), dim3(1), 0, main, words, 30000ull);
+    hipLaunchKernelGGL(lane_probe_set_kernel, dim3(1), dim3(1), 0, side, words);
+    if (hipStreamSynchronize(main) != hipSuccess || hipStreamSynchronize(side) != hipSuccess) return -1;
+    return w[1] ? 1 : 0;
   }
-  if (hipEventRecord(e1, main) != hipSuccess || hipEventSynchronize(e1) != hipSuccess) return -1.f;
-  float ms = 0.f;
-  if (hipEventElapsedTime(&ms, e0, e1) != hipSuccess) return -1.f;
-  return ms * 1e3f;
-}
-
-static bool lane_overlaps(hipStream_t main, hipStream_t side, hipEvent_t e0, hipEvent_t e1, hipEvent_t es, float alone_us) {
-  const float both = lane_probe_us(main, side, e0, e1, es);
-  return both < 0.f || both < alone_us + 33.f;      // measured: +19 us (the cross-stream event) when concurrent, +48 us on a shared hardware queue
-}
+  // (a second look where the first says no: the host may have been away for 300 us between the two launches)
+  bool overlaps(hipStream_t main, hipStream_t side) { return !words || once(main, side) != 0 || once(main, side) != 0; }
+};
 
 // (once per distinct main stream, and for at most 8 of them: a caller that rotates main streams is not probed - and synchronised - forever)
 static bool lanes_need_check(const MpmaeProgram* p, hipStream_t main) {
@@ -1081,29 +1087,17 @@ static bool lanes_need_check(const MpmaeProgram* p, hipStream_t main) {
 
 static void lanes_overlap_check(MpmaeProgram* p, hipStream_t main) {
   p->lanes_checked_for.push_back(main);
-  hipEvent_t e0 = nullptr, e1 = nullptr, es = nullptr;
-  if (hipEventCreate(&e0) != hipSuccess || hipEventCreate(&e1) != hipSuccess || hipEventCreateWithFlags(&es, hipEventDisableTiming) != hipSuccess) {
-    (void)hipGetLastError();
-    return;
-  }
+  LaneProbe probe;
   std::vector<hipStream_t> rejected;
-  (void)lane_probe_us(main, nullptr, e0, e1, es);
-  float alone = lane_probe_us(main, nullptr, e0, e1, es);
-  for (int i = 0; i < 2; ++i) { const float t = lane_probe_us(main, nullptr, e0, e1, es); if (t > 0.f && t < alone) alone = t; }
-  if (alone > 0.f) {
-    for (auto& lane : p->side) {
-      (void)lane_probe_us(main, lane, e0, e1, es);                     // warm-up (the first launch on a new stream creates its queue)
-      for (int attempt = 0; attempt < 8 && !lane_overlaps(main, lane, e0, e1, es, alone); ++attempt) {
-        hipStream_t s = nullptr;
-        if (hipStreamCreateWithFlags(&s, hipStreamNonBlocking) != hipSuccess) { (void)hipGetLastError(); break; }
-        rejected.push_back(lane);                                       // kept alive until the end: the rotation must move on
-        lane = s;
-        (void)lane_probe_us(main, lane, e0, e1, es);
-      }
+  for (auto& lane : p->side) {
+    for (int attempt = 0; attempt < 8 && !probe.overlaps(main, lane); ++attempt) {
+      hipStream_t s = nullptr;
+      if (hipStreamCreateWithFlags(&s, hipStreamNonBlocking) != hipSuccess) { (void)hipGetLastError(); break; }
+      rejected.push_back(lane);                                         // kept alive until the end: the rotation must move on
+      lane = s;
     }
   }
   for (auto s : rejected) (void)hipStreamDestroy(s);
-  (void)hipEventDestroy(e0); (void)hipEventDestroy(e1); (void)hipEventDestroy(es);
   (void)hipGetLastError();
 }
 
@@ -1113,21 +1107,10 @@ int mpmae_program_stream_overlaps(MpmaeProgram* p, mpmae_stream_t main_, mpmae_s
   hipStream_t main = S_(main_), other = S_(other_);
   if (other == main) return 0;
   if (p && !p->side.empty() && lanes_need_check(p, main)) lanes_overlap_check(p, main);
-  hipEvent_t e0 = nullptr, e1 = nullptr, es = nullptr;
-  if (hipEventCreate(&e0) != hipSuccess || hipEventCreate(&e1) != hipSuccess || hipEventCreateWithFlags(&es, hipEventDisableTiming) != hipSuccess)
-    return -(int)hipGetLastError();
-  int ok = 1;
-  std::vector<hipStream_t> against{main};
-  if (p) for (auto s : p->side) against.push_back(s);
-  for (auto a : against) {
-    (void)lane_probe_us(a, nullptr, e0, e1, es);
-    float alone = lane_probe_us(a, nullptr, e0, e1, es);
-    const float t = lane_probe_us(a, nullptr, e0, e1, es);
-    if (t > 0.f && t < alone) alone = t;
-    (void)lane_probe_us(a, other, e0, e1, es);
-    if (alone > 0.f && !lane_overlaps(a, other, e0, e1, es, alone)) ok = 0;
-  }
-  (void)hipEventDestroy(e0); (void)hipEventDestroy(e1); (void)hipEventDestroy(es);
+  LaneProbe probe;
+  if (!probe.words) return -(int)hipErrorOutOfMemory;
+  int ok = probe.overlaps(main, other);
+  if (p) for (auto lane : p->side) ok = ok && probe.overlaps(lane, other);
   (void)hipGetLastError();
   return ok;
 }

@@ -358,6 +358,26 @@ def test_lanes_and_outside_streams_are_probed_for_shared_hardware_queues():
     assert torch.isfinite(eng.total).all()
 
 
+def test_the_probe_for_shared_hardware_queues_answers_the_same_every_time():
+    """Two streams share a queue or they do not: eight answers about each of twelve streams agree (by timing, one in five was wrong), a stream that overlaps with the
+    main stream and the lanes overlaps with the main stream, and every stream picked for an exchange is such a one."""
+    import ctypes as C
+    from mmearth_train_amd import dist as mdist
+    c = CASES["allmod_atto_56"]
+    cfg = case_cfg(c)
+    sd, inputs, noise = case_data(c, cfg)
+    eng = _engine(cfg, c["N"], "bf16", sd, inputs, noise)
+    run = mdist.StepRunner(eng, world_size=1, lr=1e-4, mode="program")
+    run.step()
+    ms = C.c_void_p(torch.cuda.current_stream().cuda_stream)
+    ask = lambda prog, s: [eng.lib.mpmae_program_stream_overlaps(prog, ms, C.c_void_p(s.cuda_stream)) for _ in range(8)]  # noqa: E731
+    for s in [torch.cuda.Stream() for _ in range(12)]:
+        main, all_ = ask(None, s), ask(run.prog, s)
+        assert set(main) in ({0}, {1}) and set(all_) in ({0}, {1}) and all_[0] <= main[0], (main, all_)
+    for _ in range(3):
+        assert set(ask(run.prog, mdist.pick_concurrent_stream(eng, run.prog))) == {1}
+
+
 def test_bench_gpus_flag_starts_ranks_or_fails_loudly():
     """`python bench.py --gpus N` outside a launcher spawns N ranks itself; on a node with fewer GPUs it must refuse (exit code 2 and
     a message), not run one rank and print n_gpus: 1."""
