@@ -470,6 +470,12 @@ static int try_dwwg_mfma(const DwWgP& a, hipStream_t st, const DwWgGroupP& gr, i
   return -1;
 }
 
+// rows of partial sums -> weight and bias gradient; in fp32 as one ordered row group, so that two runs of a step agree
+static void dw_fold(int dt, const float* rows, int nrows, const MpmaeDwWgArgs& a, hipStream_t st) {
+  if (dt == 0) LAUNCH(reduce_partials_kernel<2>, dim3(cdiv(50 * a.C, 64)), dim3(256), 0, st, rows, nrows, 50 * a.C, a.dw, a.db, a.C, a.s_kh, a.s_kw, a.s_c);
+  else launch_reduce(2, rows, nrows, 50 * a.C, a.dw, a.db, a.C, a.s_kh, a.s_kw, a.s_c, st);
+}
+
 int mpmae_dwconv7_wgrad(int dt, const MpmaeDwWgArgs* a, int nblocks, mpmae_stream_t s) {
   if (!a || a->CC < 1 || a->CC > 256 || a->TP * a->g.S > 8) return (int)hipErrorInvalidValue;
   const MpmaeDwWgArgs& A = *a;      // (captured by value, as above: the group entry below passes a stack copy)
@@ -512,13 +518,16 @@ int mpmae_dwconv7_wgrad(int dt, const MpmaeDwWgArgs* a, int nblocks, mpmae_strea
     if (dt == 0) DWW5(float); else DWW5(bf16_t);
 #undef DWW5
     if (ok) {
-      launch_reduce(2, a->ws, nb, 50 * a->C, a->dw, a->db, a->C, a->s_kh, a->s_kw, a->s_c, S_(s));
+      dw_fold(dt, a->ws, nb, *a, S_(s));
       RET();
     }
   }
   const size_t lds = dw_lds_bytes(a->CC, true);
   if (lds > 160 * 1024) return (int)hipErrorInvalidValue;
   if (nblocks > a->ntiles_total) nblocks = a->ntiles_total;
+  const size_t per = (size_t)50 * a->C;
+  if (!a->ws || a->ws_floats < per || nblocks < 1) return (int)hipErrorInvalidValue;
+  if ((size_t)nblocks * per > a->ws_floats) nblocks = (int)(a->ws_floats / per);
   dim3 g(nblocks, cdiv(a->C, a->CC));
   if (dt == 0) {
     { static size_t cur = 0; if (lds > cur) { if (hipFuncSetAttribute((const void*)dwconv7_wgrad_kernel<float>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds) != hipSuccess) return (int)hipGetLastError(); cur = lds; } }
@@ -527,6 +536,7 @@ int mpmae_dwconv7_wgrad(int dt, const MpmaeDwWgArgs* a, int nblocks, mpmae_strea
     { static size_t cur = 0; if (lds > cur) { if (hipFuncSetAttribute((const void*)dwconv7_wgrad_kernel<bf16_t>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds) != hipSuccess) return (int)hipGetLastError(); cur = lds; } }
     LAUNCH(dwconv7_wgrad_kernel<bf16_t>, g, dim3(256), lds, S_(s), A);
   }
+  dw_fold(dt, a->ws, nblocks, *a, S_(s));
   RET();
 }
 

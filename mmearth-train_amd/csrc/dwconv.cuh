@@ -168,21 +168,19 @@ __global__ __launch_bounds__(256) void dwconv7_wgrad_kernel(const DwWgP q) {
   __syncthreads();
   for (int i = threadIdx.x; i < 50 * CC; i += blockDim.x) red[i] = 0.f;
   __syncthreads();
-  if (tg < ngroups && c < C) {
+  // One row of partial sums per workgroup, groups and rows added in a fixed order: by atomics, a gradient that is zero but for roundings came out different on every
+  // run, by more than the optimizer's eps.
+  for (int gi = 0; gi < ngroups; ++gi) {
+    if (tg == gi && c < C) {
 #pragma unroll
-    for (int k = 0; k < 49; ++k) atomicAdd(&red[k * CC + tc], adw[k]);
-    atomicAdd(&red[49 * CC + tc], adb);
+      for (int k = 0; k < 49; ++k) red[k * CC + tc] += adw[k];
+      red[49 * CC + tc] += adb;
+    }
+    __syncthreads();
   }
-  __syncthreads();
+  float* out = q.ws + (size_t)blockIdx.x * 50 * C;
   for (int i = threadIdx.x; i < 50 * CC; i += blockDim.x) {
     const int k = i / CC, cc = i - k * CC;
-    if (c0 + cc >= C) continue;
-    const float v = red[i];
-    if (k < 49) {
-      const int kh = k / 7, kw = k - kh * 7;
-      atomicAdd(q.dw + kh * q.s_kh + kw * q.s_kw + (c0 + cc) * q.s_c, v);
-    } else if (q.db) {
-      atomicAdd(q.db + c0 + cc, v);
-    }
+    if (c0 + cc < C) out[(size_t)k * C + c0 + cc] = red[i];
   }
 }

@@ -333,6 +333,31 @@ def test_rccl_exchange_runs_at_world_size_one():
         assert re.search(mode + r": exposed communication tail [0-9.]+ ms per step", r.stdout), r.stdout      # StepRunner.measure_comm_tail
 
 
+def test_fp32_depthwise_gradients_do_not_depend_on_the_run():
+    """The weight and bias gradients of every depthwise convolution, in fp32, are sums in a fixed order: bit for bit the same on every run of the same step. (By atomics
+    the one element of this batch that is zero but for roundings, about 1e-8, varied by 1.5e-8: AdamW's first update, lr g / (|g| + 1e-8), varied with it.)"""
+    from mmearth_train_amd import dist as mdist
+    from mmearth_train_amd.config import make_cfg
+    from mmearth_train_amd.synth import make_inputs, make_state_dict
+    cfg = make_cfg()
+    sd, (inputs, noise) = make_state_dict(cfg, seed=5), make_inputs(cfg, 4, seed=6)
+    first = None
+    for _ in range(4):
+        eng = _engine(cfg, 4, "f32", sd, inputs, noise)
+        run = mdist.StepRunner(eng, world_size=1, lr=1e-3, mode="program")
+        run.step()
+        torch.cuda.synchronize()
+        flat, got = eng.gflat.clone(), {}
+        for name, p in eng.params.items():
+            if "dwconv" in name:
+                o = eng.offsets[name]
+                o = o[0] if isinstance(o, (tuple, list)) else o
+                got[name] = flat[o:o + p.numel()]
+        assert len(got) > 20 and all(bool(g.any()) for g in got.values())
+        first = first or got
+        assert all(torch.equal(first[k], g) for k, g in got.items()), [k for k, g in got.items() if not torch.equal(first[k], g)]
+
+
 def test_lanes_and_outside_streams_are_probed_for_shared_hardware_queues():
     """ROCm serialises HIP streams that share a hardware queue. The launch program probes its side lanes against the main stream at the
     first replay (and replaces a colliding lane); mpmae_program_stream_overlaps answers the same question for a stream outside the program.
