@@ -257,3 +257,21 @@ def test_xcd_tile_order_is_a_permutation_that_keeps_a_row_tile_on_one_xcd():
                 assert len({c for c, _, _ in lst}) == 1, (gx, gy, m)                      # one XCD
                 js = sorted(j for _, j, _ in lst)
                 assert js == list(range(js[0], js[0] + gy)), (gx, gy, m)                  # back to back on it
+
+
+def test_no_unit_holds_packed_fp32_instructions(tmp_path):
+    """The build switches them off for every unit; the device code of the library as it is built has none."""
+    import shutil
+    from mmearth_train_amd import _lib
+    _lib.load()
+    objdump = "/opt/rocm/llvm/bin/llvm-objdump"
+    if not os.path.isfile(objdump):
+        pytest.skip("no llvm-objdump")
+    lib = shutil.copy(_lib.LIB_PATH, tmp_path)
+    subprocess.run([objdump, "--offloading", lib], check=True, capture_output=True, cwd=tmp_path)
+    parts = [p for p in os.listdir(tmp_path) if "gfx950" in p]
+    assert parts
+    for p in parts:
+        with subprocess.Popen([objdump, "-d", str(tmp_path / p)], stdout=subprocess.PIPE, text=True) as run:
+            found = [line.strip() for line in run.stdout if "v_pk_" in line and any(op in line for op in ("v_pk_add_f32", "v_pk_mul_f32", "v_pk_fma_f32"))]
+        assert run.returncode == 0 and not found, (p, found[:3])
