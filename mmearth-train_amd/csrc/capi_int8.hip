@@ -26,10 +26,10 @@ static void quant_rows(const T* x, long long ldx, int M, int K, int8_t* q, int l
   if (K & 7) quant_rows_of<T, true>(x, ldx, M, K, q, ldq, scale, st);
   else quant_rows_of<T, false>(x, ldx, M, K, q, ldq, scale, st);
 }
-template <typename T, int MT, int NT, bool FUSED>
+template <typename T, bool FUSED>
 static void skinny(const MpmaeI8Args& a, hipStream_t st) {
-  const size_t lds = (size_t)8 * MT * NT * 1024 + (FUSED ? (size_t)a.M * (a.ldq + 16) : 0);
-  LAUNCH((i8_skinny_kernel<T, MT, NT, FUSED>), dim3(cdiv(a.N, 16 * NT)), dim3(512), lds, st, (const T*)a.x, a.ldx, (const int8_t*)a.q, (const float*)a.sx, a.w, a.sw,
+  const size_t lds = 8 * 1024 + (FUSED ? (size_t)a.M * (a.ldq + 16) : 0);
+  LAUNCH((i8_skinny_kernel<T, FUSED>), dim3(cdiv(a.N, 16)), dim3(512), lds, st, (const T*)a.x, a.ldx, (const int8_t*)a.q, (const float*)a.sx, a.w, a.sw,
          a.bias, (T*)a.y, a.ldy, a.M, a.N, a.K, a.ldq);
 }
 template <typename T, int BM, int BN, int WM, int WN, int BK, int ST>
@@ -55,12 +55,12 @@ template <typename T>
 static void linear_i8(const MpmaeI8Args& a, hipStream_t st) {
   // Up to 8 rows of a moderate length: one launch that quantises and multiplies (1 x 1024 -> 4096: 4.8 us; 7.2 us in two launches). A workgroup holds the rows in
   // its registers; longer ones go through a launch of their own.
-  if (a.M <= 8 && i8_vectors(a.M, a.ldq) <= I8_KEPT && a.K >= 8) return skinny<T, 1, 1, true>(a, st);
+  if (a.M <= 8 && i8_vectors(a.M, a.ldq) <= I8_KEPT && a.K >= 8) return skinny<T, true>(a, st);
   quant_rows((const T*)a.x, a.ldx, a.M, a.K, a.q, a.ldq, a.sx, st);
   auto count = [&](int bm, int bn) { return (long long)cdiv(a.M, bm) * cdiv(a.N, bn); };
   const int splits = i8_splits(a.M, a.N, a.ldq);
   // 16 x 2816 -> 1000: 4.3 us with k split between the waves, 7.1 us in 32 x 64 tiles; -> 11264: 11.4 and 7.9 us
-  if (i8_few(a.M, a.N)) return skinny<T, 1, 1, false>(a, st);
+  if (i8_few(a.M, a.N)) return skinny<T, false>(a, st);
   if (splits > 1) {
     const int mt = cdiv(a.M, 32), nt = cdiv(a.N, 64);
     LAUNCH((i8_tile_kernel<T, 32, 64, 2, 2, 128, 4, true>), dim3(mt * nt, splits), dim3(256), i8_tile_lds(32, 64, 128, 4), st, (const int8_t*)a.q, (const float*)a.sx, a.w, a.sw,

@@ -13,9 +13,6 @@
 #include <type_traits>
 
 #define I8_KPAD 128
-#ifndef I8_PIPE
-#define I8_PIPE 1
-#endif
 typedef __attribute__((ext_vector_type(4))) int i32x4_t;
 
 // Eight elements of a row of at least eight from element i on: one load from a clamped address (a load behind a branch is waited for where the branch joins,
@@ -150,7 +147,7 @@ __global__ __launch_bounds__(256) void i8_quant_kernel(const T* __restrict__ x, 
 }
 
 // ---------------------------------------------------------------------------------
-// Up to MT * 16 rows: bound by reading W once. A workgroup of eight waves takes 16 * NT columns and splits k between the waves, so that even a
+// Up to 16 rows: bound by reading W once. A workgroup of eight waves takes 16 columns and splits k between the waves, so that even a
 // layer of 1000 columns has every load of W in flight at once; the eight integer partial sums meet in LDS. A wave's step is 128 bytes of k
 // (two matrix operands of 64), so that every row of W is read in whole 128-byte lines. D[n][m] = W x^T: a lane ends with four consecutive columns of one row.
 // FUSED: every workgroup quantises the rows itself, into LDS (x is small and in L2; the launch and the wait of a kernel of its own cost more).
@@ -197,32 +194,28 @@ __device__ __forceinline__ void i8_quant_kept(const T* __restrict__ x, long long
   }
   __syncthreads();
 }
-template <typename T, int MT, int NT, bool FUSED>
+template <typename T, bool FUSED>
 __global__ __launch_bounds__(512) void i8_skinny_kernel(const T* __restrict__ x, long long ldx, const int8_t* __restrict__ A, const float* __restrict__ sa,
                                                         const int8_t* __restrict__ B, const float* __restrict__ sb, const float* __restrict__ bias,
                                                         T* __restrict__ y, long long ldy, int M, int N, int K, int Kp) {
   extern __shared__ __attribute__((aligned(16))) unsigned char i8_smem[];
-  int* red = reinterpret_cast<int*>(i8_smem);                                             // [8][MT * NT][16 m][16 n]
-  int8_t* Al = reinterpret_cast<int8_t*>(i8_smem) + 8 * MT * NT * 1024;                    // [M][Kp + 16] (FUSED)
-  __shared__ unsigned smax[16][8];
-  __shared__ float ssx[16];
+  int* red = reinterpret_cast<int*>(i8_smem);                                             // [8][16 m][16 n]
+  int8_t* Al = reinterpret_cast<int8_t*>(i8_smem) + 8 * 1024;                             // [M][Kp + 16] (FUSED)
+  __shared__ unsigned smax[8][8];
+  __shared__ float ssx[8];
   // (matrix instructions ignore the lane mask: what decides whether a wave runs them is a scalar)
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lr = lane & 15, lg = lane >> 4;
-  const int n0 = blockIdx.x * 16 * NT;
+  const int n0 = blockIdx.x * 16;
   const int steps = Kp >> 7;
-  const int8_t* b[NT];
-#pragma unroll
-  for (int j = 0; j < NT; ++j) b[j] = B + (size_t)min(n0 + j * 16 + lr, N - 1) * Kp + lg * 16;
-  constexpr int U = MT == 1 ? 4 : 2;                        // steps whose loads are in flight together
-  i32x4_t bv[U][NT][2];
+  const int8_t* b = B + (size_t)min(n0 + lr, N - 1) * Kp + lg * 16;
+  constexpr int U = 4;                                      // steps whose loads are in flight together
+  i32x4_t bv[U][2];
   auto load_w = [&](int s0) {
 #pragma unroll
     for (int u = 0; u < U; ++u)
       if (s0 + u * 8 < steps) {
 #pragma unroll
-        for (int j = 0; j < NT; ++j)
-#pragma unroll
-          for (int h = 0; h < 2; ++h) bv[u][j][h] = *reinterpret_cast<const i32x4_t*>(b[j] + ((s0 + u * 8) << 7) + h * 64);
+        for (int h = 0; h < 2; ++h) bv[u][h] = *reinterpret_cast<const i32x4_t*>(b + ((s0 + u * 8) << 7) + h * 64);
       }
   };
   load_w(w);                                                // the first weights are on their way while x is quantised
@@ -233,49 +226,34 @@ __global__ __launch_bounds__(512) void i8_skinny_kernel(const T* __restrict__ x,
     else if (two) i8_quant_kept<T, 2, false>(x, ldx, M, K, Al, Kp, ssx, smax);
     else i8_quant_kept<T, I8_KEPT, false>(x, ldx, M, K, Al, Kp, ssx, smax);
   }
-  const int8_t* a[MT];
-#pragma unroll
-  for (int i = 0; i < MT; ++i) {
-    const int r = min(i * 16 + lr, M - 1);
-    a[i] = (FUSED ? Al + (size_t)r * (Kp + 16) : A + (size_t)r * Kp) + lg * 16;
-  }
-  i32x4_t acc[MT][NT] = {};
+  const int r = min(lr, M - 1);
+  const int8_t* a = (FUSED ? Al + (size_t)r * (Kp + 16) : A + (size_t)r * Kp) + lg * 16;
+  i32x4_t acc = {};
   for (int s0 = w; s0 < steps; s0 += 8 * U) {
     if (s0 != w) load_w(s0);
-    i32x4_t av[U][MT][2];
+    i32x4_t av[U][2];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       if (s0 + u * 8 < steps) {
-        const int k = (s0 + u * 8) << 7;
 #pragma unroll
-        for (int i = 0; i < MT; ++i)
-#pragma unroll
-          for (int h = 0; h < 2; ++h) av[u][i][h] = *reinterpret_cast<const i32x4_t*>(a[i] + k + h * 64);
+        for (int h = 0; h < 2; ++h) av[u][h] = *reinterpret_cast<const i32x4_t*>(a + ((s0 + u * 8) << 7) + h * 64);
       }
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       if (s0 + u * 8 < steps) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-          for (int i = 0; i < MT; ++i)
-#pragma unroll
-            for (int j = 0; j < NT; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(bv[u][j][h], av[u][i][h], acc[i][j], 0, 0, 0);
+        for (int h = 0; h < 2; ++h) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(bv[u][h], av[u][h], acc, 0, 0, 0);
       }
     }
   }
-  // lane: row i * 16 + lr, columns j * 16 + lg * 4 .. + 3
-#pragma unroll
-  for (int i = 0; i < MT; ++i)
-#pragma unroll
-    for (int j = 0; j < NT; ++j) *reinterpret_cast<i32x4_t*>(red + ((w * MT * NT + i * NT + j) * 16 + lr) * 16 + lg * 4) = acc[i][j];
+  *reinterpret_cast<i32x4_t*>(red + (w * 16 + lr) * 16 + lg * 4) = acc;      // lane: row lr, columns lg * 4 .. + 3
   __syncthreads();
-  for (int o = threadIdx.x; o < MT * NT * 256; o += 512) {
+  if (threadIdx.x < 256) {
+    const int o = threadIdx.x, m = o >> 4, n = n0 + (o & 15);
     int sum = 0;
 #pragma unroll
-    for (int v = 0; v < 8; ++v) sum += red[v * MT * NT * 256 + o];
-    const int tile = o >> 8, m = (tile / NT) * 16 + ((o >> 4) & 15), n = n0 + (tile % NT) * 16 + (o & 15);
+    for (int v = 0; v < 8; ++v) sum += red[v * 256 + o];
     if (m < M && n < N) elem_st(y + (size_t)m * ldy + n, i8_out(sum, FUSED ? ssx[m] : sa[m], sb[n], bias ? bias[n] : 0.f));
   }
 }
@@ -392,7 +370,7 @@ __global__ __launch_bounds__(WM * WN * 64, i8_waves_per_simd(i8_tile_lds(BM, BN,
     }
   }
   int slot = 0;
-  if constexpr (KS == 2 && I8_PIPE) {
+  if constexpr (KS == 2) {
     // the fragments of the next half slab are read under the products of the current one, across the barrier too
     i32x4_t bf[2][TN], af[2][TM];
     ready(0);
