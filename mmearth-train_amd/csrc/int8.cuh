@@ -420,7 +420,12 @@ __global__ __launch_bounds__(WM * WN * 64, i8_waves_per_simd(i8_tile_lds(BM, BN,
     }
     return;
   }
-  // y goes past the caches where its pieces of 64 bytes are whole (50176 x 512 -> 2048: 82 -> 76 us); pieces that straddle need the cache to be put together
+  // y goes past the caches where its pieces of 64 bytes are whole; pieces that straddle need the cache to be put together. us of the layer, in brackets with a GELU
+  // that reads y behind it, past the caches / through them:
+  //   bf16  1568 x 512 -> 2048 (6.4 MB) 10.9 (17.8) / 11.3 (18.6)    3136 x 640 -> 2560 (16 MB) 17.4 (29.2) / 18.3 (30.4)    12544 x 512 -> 2048 (51 MB) 35.0 (58.5) / 35.1 (58.4)
+  //         12544 x 1024 -> 4096 (103 MB) 77.4 (122) / 81.0 (125)    50176 x 512 -> 2048 (206 MB) 93.7 (185) / 101 (194)    200704 x 80 -> 320 (129 MB) 55.6 (108) / 53.0 (107)
+  //   fp32  784 x 640 -> 2560 (8 MB) 10.7 (16.1) / 11.0 (17.2)       3136 x 320 -> 1280 (16 MB) 12.4 (22.4) / 13.0 (23.5)    12544 x 320 -> 1280 (64 MB) 28.8 (46.5) / 27.8 (46.7)
+  //         50176 x 160 -> 640 (129 MB) 51.7 (84.0) / 41.6 (83.8): what a layer alone gains there, its reader pays
   const bool past = ((((uintptr_t)y) | ((uintptr_t)ldy * sizeof(T))) & 63) == 0;
 #pragma unroll
   for (int jp = 0; jp < TN / 2; ++jp) {
