@@ -67,6 +67,7 @@ PyObject* gather(PyObject*, PyObject* args) {
         if (p.layout() != at::kStrided || p.device().index() != device || p.device().is_cuda() != (device >= 0)) wrong = "has left the optimizer's device";
         else if (p.numel() != want[i].n || code_of(p.scalar_type()) != want[i].dt) wrong = "has another size or type than when the optimizer first ran";
         else if (!p.is_non_overlapping_and_dense()) wrong = "is not dense in memory";
+        else if (p.is_inference()) wrong = "was made in inference mode: it has no version to count";
         else if (orders[i] && orders[i] != order_of(p)) wrong = "has its elements in another order than when the optimizer first ran";
         else if (const at::Tensor& g = p.grad(); g.defined()) {
           if (g.layout() != at::kStrided) wrong = "has a sparse gradient";

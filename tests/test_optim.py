@@ -175,6 +175,23 @@ def test_lists_are_compared_object_for_object():
         same([], [], 3)
 
 
+def test_a_parameter_of_inference_mode_is_refused_before_anything_is_written():
+    """It has no version counter, and the error that counting it raises would come half way through the list."""
+    from mmearth_train_amd import _lib
+    host = _lib.host_tensors()
+    with torch.inference_mode():
+        second = torch.nn.Parameter(torch.ones(7))
+        second.grad = torch.ones(7)
+    params = [torch.nn.Parameter(torch.ones(300)), second]
+    params[0].grad = torch.ones(300)
+    table, out, orders = _reader_state(params)
+    keep = table.copy()
+    params[0].data = params[0].data.clone()
+    with pytest.raises(ValueError, match="parameter 1 was made in inference mode"):
+        host.gather(params, table.ctypes.data, -1, out.ctypes.data, orders.ctypes.data, True)
+    assert np.array_equal(table, keep) and not orders.any() and params[0]._version == 0
+
+
 @pytest.fixture(scope="module")
 def lib():
     from mmearth_train_amd import _lib
