@@ -24,8 +24,9 @@ namespace {
 
 int code_of(at::ScalarType t) { return t == at::kFloat ? 0 : t == at::kBFloat16 ? 1 : t == at::kHalf ? 2 : -1; }
 
-// same element order in memory: equal strides wherever a dimension has more than one element
+// same element order in memory: equal strides wherever a dimension has more than one element, and the memory holds the values themselves (no negated view)
 bool same_order(const at::Tensor& a, const at::Tensor& b) {
+  if (b.is_neg()) return false;
   const auto sa = a.strides(), sb = b.strides(), n = a.sizes();
   for (size_t i = 0; i < n.size(); ++i)
     if (n[i] != 1 && sa[i] != sb[i]) return false;
@@ -66,7 +67,7 @@ PyObject* gather(PyObject*, PyObject* args) {
         const at::Tensor& p = THPVariable_Unpack(o);
         if (p.layout() != at::kStrided || p.device().index() != device || p.device().is_cuda() != (device >= 0)) wrong = "has left the optimizer's device";
         else if (p.numel() != want[i].n || code_of(p.scalar_type()) != want[i].dt) wrong = "has another size or type than when the optimizer first ran";
-        else if (!p.is_non_overlapping_and_dense()) wrong = "is not dense in memory";
+        else if (!p.is_non_overlapping_and_dense() || p.is_neg()) wrong = "is not dense in memory";
         else if (p.is_inference()) wrong = "was made in inference mode: it has no version to count";
         else if (orders[i] && orders[i] != order_of(p)) wrong = "has its elements in another order than when the optimizer first ran";
         else if (const at::Tensor& g = p.grad(); g.defined()) {

@@ -192,6 +192,21 @@ def test_a_parameter_of_inference_mode_is_refused_before_anything_is_written():
     assert np.array_equal(table, keep) and not orders.any() and params[0]._version == 0
 
 
+def test_a_negated_gradient_is_copied_not_addressed():
+    """The imaginary part of a conjugate: its memory holds the values with the other sign."""
+    from mmearth_train_amd import _lib
+    host = _lib.host_tensors()
+    p = torch.nn.Parameter(torch.ones(1))
+    p.grad = torch.tensor([1 + 2j]).conj().imag
+    assert p.grad.is_neg() and float(p.grad) == -2.0
+    table, out, orders = _reader_state([p])
+    assert host.gather([p], table.ctypes.data, -1, out.ctypes.data, orders.ctypes.data, True) == (1, False, [0]) and out[0] == 0
+    q = torch.nn.Parameter(torch.tensor([1 + 2j]).conj().imag.detach())
+    if q.is_neg():
+        with pytest.raises(ValueError, match="dense"):
+            host.gather([q], table.ctypes.data, -1, out.ctypes.data, np.zeros(1, np.uint64).ctypes.data, True)
+
+
 @pytest.fixture(scope="module")
 def lib():
     from mmearth_train_amd import _lib
