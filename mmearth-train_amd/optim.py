@@ -311,8 +311,12 @@ class AdamW(torch.optim.Optimizer):
         ids = [i for g in groups for i in g["params"]]
         entries = [state_dict["state"].get(i) for i in ids]
         for (shape, _), st in zip(plan.shapes, entries):
-            if st is not None and (st["exp_avg"].shape != shape or st["exp_avg_sq"].shape != shape):
-                raise ValueError(f"loaded moments of shape {tuple(st['exp_avg'].shape)} for a parameter of shape {tuple(shape)}")
+            for key in ("exp_avg", "exp_avg_sq") if st is not None else ():
+                if not isinstance(st.get(key), torch.Tensor) or st[key].shape != shape or st[key].is_complex():
+                    raise ValueError(f"loaded {key} is {getattr(st.get(key), 'shape', None)} for a parameter of shape {tuple(shape)}")
+        steps = [0 if st is None else float(st.get("step", -1)) for st in entries]
+        if not all(0 <= t < 2 ** 31 and t == int(t) for t in steps):
+            raise ValueError(f"loaded step counts are whole numbers from 0 on: {steps}")
         for mine, g in zip(self.param_groups, groups):
             mine.update({k: v for k, v in g.items() if k in self.defaults or k not in _TORCH_ONLY})
         into = [plan.m, plan.v] if self.state_bits == 32 else [torch.zeros(plan.size, device=plan.device) for _ in range(2)]
@@ -326,7 +330,7 @@ class AdamW(torch.optim.Optimizer):
                 torch._foreach_zero_(absent)
         if self.state_bits == 8:
             plan.store(*into)
-        plan.steps.copy_(torch.tensor([0 if st is None else int(float(st["step"])) for st in entries], dtype=torch.int32))
+        plan.steps.copy_(torch.tensor([int(t) for t in steps], dtype=torch.int32))
 
     def __getstate__(self):
         raise TypeError("the state lives in device buffers: use state_dict()")

@@ -713,3 +713,31 @@ def test_a_group_added_on_another_stream(bits):
     fill = [torch.full_like(x, 7.0) for x in (m, v) for _ in range(2)]
     assert all(torch.equal(x[:5_000_000], y[:5_000_000]) for x, y in zip((m, v), opt.flat_moments())) and len(fill) == 4
     assert opt.plan.steps.tolist() == [1, 0]
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_refused_checkpoint_changes_nothing(bits):
+    from mmearth_train_amd.optim import AdamW
+    params = params_of([300, 700], DT[:1], 25)
+    opt = AdamW(params, lr=1e-3, state_bits=bits)
+    grads_for(params, 140)
+    opt.step()
+    keep = [x.clone() for x in opt.flat_moments()]
+
+    def spoiled(i, key, value):
+        sd = opt.state_dict()
+        sd["param_groups"][0]["lr"] = 5.0
+        for st in sd["state"].values():
+            st["exp_avg"] = st["exp_avg"] + 1.0
+        if value is None:
+            del sd["state"][i][key]
+        else:
+            sd["state"][i][key] = value
+        return sd
+
+    for i, key, value in ((1, "step", None), (1, "step", torch.tensor(float("nan"))), (1, "step", -1), (0, "step", 2.5), (1, "step", 2.0 ** 31), (1, "exp_avg_sq", None),
+                          (1, "exp_avg_sq", torch.zeros(699, device="cuda")), (0, "exp_avg", 3.0), (0, "exp_avg", torch.zeros(300, dtype=torch.complex64))):
+        with pytest.raises(ValueError, match="loaded"):
+            opt.load_state_dict(spoiled(i, key, value))
+        assert opt.param_groups[0]["lr"] == 1e-3 and opt.plan.steps.tolist() == [1, 1]
+        assert all(torch.equal(a, b) for a, b in zip(keep, opt.flat_moments())), (i, key)
