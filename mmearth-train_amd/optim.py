@@ -284,6 +284,8 @@ class AdamW(torch.optim.Optimizer):
     def state_dict(self):
         """torch.optim.AdamW.state_dict() layout: per-parameter step / exp_avg / exp_avg_sq, fp32, all copies (an optimizer that
         loads them keeps the tensors it is given). With 8 bits they are the values of the codes, and loading them gives the same codes again."""
+        for hook in self._optimizer_state_dict_pre_hooks.values():
+            hook(self)
         groups, at = [], 0
         for g in self.param_groups:
             groups.append({**{k: v for k, v in g.items() if k != "params"}, "amsgrad": False, "maximize": False, "foreach": None, "capturable": False,
@@ -295,11 +297,18 @@ class AdamW(torch.optim.Optimizer):
             for i, (m, v) in enumerate(zip(*map(plan.views, plan.values()))):
                 if steps[i]:
                     state[i] = {"step": torch.tensor(float(steps[i])), "exp_avg": m.clone(), "exp_avg_sq": v.clone()}
-        return {"state": state, "param_groups": groups}
+        out = {"state": state, "param_groups": groups}
+        for hook in self._optimizer_state_dict_post_hooks.values():
+            done = hook(self, out)
+            out = out if done is None else done
+        return out
 
     @torch.no_grad()
     def load_state_dict(self, state_dict):
         """What this class or torch.optim.AdamW wrote for the same parameter groups."""
+        for hook in self._optimizer_load_state_dict_pre_hooks.values():
+            done = hook(self, state_dict)
+            state_dict = state_dict if done is None else done
         groups = state_dict["param_groups"]
         if [len(g["params"]) for g in groups] != [len(g["params"]) for g in self.param_groups]:
             raise ValueError("loaded state dict has other parameter groups than the optimizer")
@@ -331,6 +340,8 @@ class AdamW(torch.optim.Optimizer):
         if self.state_bits == 8:
             plan.store(*into)
         plan.steps.copy_(torch.tensor([int(t) for t in steps], dtype=torch.int32))
+        for hook in self._optimizer_load_state_dict_post_hooks.values():
+            hook(self)
 
     def __getstate__(self):
         raise TypeError("the state lives in device buffers: use state_dict()")

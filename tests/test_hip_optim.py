@@ -741,3 +741,17 @@ def test_a_refused_checkpoint_changes_nothing(bits):
             opt.load_state_dict(spoiled(i, key, value))
         assert opt.param_groups[0]["lr"] == 1e-3 and opt.plan.steps.tolist() == [1, 1]
         assert all(torch.equal(a, b) for a, b in zip(keep, opt.flat_moments())), (i, key)
+
+
+def test_hooks_of_checkpoints_run():
+    from mmearth_train_amd.optim import AdamW
+    params = params_of([30], DT[:1], 26)
+    opt, seen = AdamW(params), []
+    grads_for(params, 150)
+    opt.step()
+    opt.register_state_dict_pre_hook(lambda o: seen.append("before"))
+    opt.register_state_dict_post_hook(lambda o, sd: {**sd, "note": 3})
+    opt.register_load_state_dict_pre_hook(lambda o, sd: (seen.append(sd["note"]), {k: v for k, v in sd.items() if k != "note"})[1])
+    opt.register_load_state_dict_post_hook(lambda o: seen.append("after"))
+    opt.load_state_dict(opt.state_dict())
+    assert seen == ["before", 3, "after"] and opt.plan.steps.tolist() == [1]
