@@ -146,8 +146,12 @@ class AdamW(torch.optim.Optimizer):
             raise ValueError(f"max_norm is a positive number or None, not {max_norm!r}")
         defaults = dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay)
         self._check_group(defaults)
-        self.state_bits, self.max_norm, self._plan = state_bits, max_norm, None
+        self._state_bits, self._max_norm, self._plan = state_bits, max_norm, None
         super().__init__(params, defaults)
+
+    # (both are built into the state and its launches: set on an optimizer that runs, they would do nothing)
+    state_bits = property(lambda self: self._state_bits)
+    max_norm = property(lambda self: self._max_norm)
 
     @staticmethod
     def _check_group(g):

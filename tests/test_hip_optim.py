@@ -755,3 +755,13 @@ def test_hooks_of_checkpoints_run():
     opt.register_load_state_dict_post_hook(lambda o: seen.append("after"))
     opt.load_state_dict(opt.state_dict())
     assert seen == ["before", 3, "after"] and opt.plan.steps.tolist() == [1]
+
+
+def test_settings_of_the_whole_optimizer_are_fixed():
+    from mmearth_train_amd.optim import AdamW
+    opt = AdamW(params_of([30], DT[:1], 27), state_bits=8, max_norm=0.5)
+    assert opt.state_bits == 8 and opt.max_norm == 0.5
+    for name, value in (("max_norm", 1.0), ("state_bits", 32)):
+        with pytest.raises(AttributeError):
+            setattr(opt, name, value)
+    assert opt.state_bits == 8 and opt.max_norm == 0.5
