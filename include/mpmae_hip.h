@@ -589,7 +589,7 @@ int mpmae_sumsq(const float* x, size_t n, float* out, mpmae_stream_t stream);
  * A tensor without a gradient (NULL) is left alone and its step count stands; so does everything when the norm, in fp32, is not finite (norm_skip[1] = 1).
  * Steps are counted on the device, so a captured call replays as the next step.
  *   - grads (HOST): gradient address of every tensor, passed to the kernels by value; in the parameter's own dense element order;
- *   - groups (HOST): {lr, beta1, beta2, eps, weight_decay} of every parameter group;
+ *   - groups (HOST): {lr, beta1, beta2, eps, weight_decay} of every parameter group; finite, not negative, betas below 1 (hipErrorInvalidValue);
  *   - tensors (device, MpmaeAdamwTensor[nt]), chunks (device, int pairs {tensor, index} of every 2048-element piece, by tensor), chunk_first (HOST, nt + 1):
  *     the static description; off is the tensor's first element in the moment buffers, a multiple of 256, so is every buffer's length;
  *   - bits = 32: m, v fp32. bits = 8: m int8 / v uint8 codes and one fp32 scale per 256 elements (ms, vs): m = ms k|k| / 127^2, v = vs (k / 255)^4.

@@ -13,6 +13,11 @@ int mpmae_adamw_multi(const MpmaeAdamwArgs* a, const void* const* grads, const d
   if (!a || !grads || !groups || ngroups < 1 || a->nt < 1 || !a->tensors || !a->chunks || !a->chunk_first || !a->steps || !a->hyper ||
       !a->m || !a->v || (a->bits != 8 && a->bits != 32) || (a->bits == 8 && (!a->ms || !a->vs)) || (a->max_norm > 0 && (!a->partials || !a->norm_skip)))
     return (int)hipErrorInvalidValue;
+  for (int g = 0; g < ngroups; ++g) {
+    const double* h = groups + 5 * (size_t)g;
+    if (!(h[0] >= 0 && h[0] < INFINITY && h[1] >= 0 && h[1] < 1 && h[2] >= 0 && h[2] < 1 && h[3] >= 0 && h[3] < INFINITY && h[4] >= 0 && h[4] < INFINITY))
+      return (int)hipErrorInvalidValue;      // (a beta of 1 divides by 1 - 1^t)
+  }
   const AdamwTensor* tensors = reinterpret_cast<const AdamwTensor*>(a->tensors);
   const int2* chunks = reinterpret_cast<const int2*>(a->chunks);
   const bool clip = a->max_norm > 0;

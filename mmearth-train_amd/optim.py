@@ -281,7 +281,12 @@ class AdamW(torch.optim.Optimizer):
                 raise ValueError("lr is a number: a tensor would have to be read back on every step")
             groups += (g["lr"], *g["betas"], g["eps"], g["weight_decay"])
         hyper = (C.c_double * len(groups))(*groups)
-        plan.launch("adamw_multi", lambda stream: _lib.load().mpmae_adamw_multi(plan.ref, plan.grads_at, hyper, len(self.param_groups), stream))
+        try:
+            plan.launch("adamw_multi", lambda stream: _lib.load().mpmae_adamw_multi(plan.ref, plan.grads_at, hyper, len(self.param_groups), stream))
+        except _lib.HipLibraryError:
+            for g in self.param_groups:                # (what the native call refuses, in words)
+                self._check_group(g)
+            raise
         return loss
 
     # ---- checkpoints: torch.optim.AdamW's layout -------------------------------------------------------------------------------------------

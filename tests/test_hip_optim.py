@@ -765,3 +765,21 @@ def test_settings_of_the_whole_optimizer_are_fixed():
         with pytest.raises(AttributeError):
             setattr(opt, name, value)
     assert opt.state_bits == 8 and opt.max_norm == 0.5
+
+
+def test_settings_changed_to_impossible_ones_are_refused():
+    from mmearth_train_amd.optim import AdamW
+    params = params_of([300], DT[:1], 28)
+    opt = AdamW(params, lr=1e-3)
+    grads_for(params, 160)
+    opt.step()
+    keep = params[0].detach().clone()
+    for key, value, what in (("betas", (1.0, 0.999), "betas"), ("lr", float("nan"), "lr"), ("lr", -1.0, "lr"), ("eps", float("inf"), "eps"), ("weight_decay", -1.0, "weight_decay")):
+        old = opt.param_groups[0][key]
+        opt.param_groups[0][key] = value
+        with pytest.raises(ValueError, match=what):
+            opt.step()
+        opt.param_groups[0][key] = old
+        assert torch.equal(keep, params[0].detach()) and opt.plan.steps.tolist() == [1]
+    opt.step()
+    assert opt.plan.steps.tolist() == [2]

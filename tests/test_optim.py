@@ -207,6 +207,19 @@ def test_a_negated_gradient_is_copied_not_addressed():
             host.gather([q], table.ctypes.data, -1, out.ctypes.data, np.zeros(1, np.uint64).ctypes.data, True)
 
 
+def test_library_refuses_settings_that_no_update_has(lib):
+    """hipErrorInvalidValue is 1; what is let through fails here for want of a GPU, with another error."""
+    from mmearth_train_amd import _lib
+    some = C.create_string_buffer(256)
+    at = C.addressof(some)
+    args = _lib.AdamwArgs(tensors=at, chunks=at, chunk_first=at, steps=at, hyper=at, partials=at, norm_skip=at, m=at, v=at, ms=at, vs=at, max_norm=0.0, nt=1, npartials=1, bits=32)
+    nan, inf = float("nan"), float("inf")
+    for bad in ((-1e-3, 0.9, 0.99, 1e-8, 0.0), (nan, 0.9, 0.99, 1e-8, 0.0), (inf, 0.9, 0.99, 1e-8, 0.0), (1e-3, 1.0, 0.99, 1e-8, 0.0), (1e-3, 0.9, 1.0, 1e-8, 0.0),
+                (1e-3, -0.1, 0.99, 1e-8, 0.0), (1e-3, 0.9, nan, 1e-8, 0.0), (1e-3, 0.9, 0.99, -1e-8, 0.0), (1e-3, 0.9, 0.99, 1e-8, inf)):
+        groups = (C.c_double * 10)(1e-3, 0.9, 0.99, 1e-8, 0.0, *bad)
+        assert lib.mpmae_adamw_multi(C.byref(args), at, groups, 2, None) == 1, bad
+
+
 @pytest.fixture(scope="module")
 def lib():
     from mmearth_train_amd import _lib
