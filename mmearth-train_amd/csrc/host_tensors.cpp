@@ -18,6 +18,7 @@
 #include <exception>
 #include <optional>
 #include <tuple>
+#include <vector>
 #include "../../include/mpmae_hip.h"
 
 namespace {
@@ -59,49 +60,56 @@ PyObject* gather(PyObject*, PyObject* args) {
   PyObject* other = nullptr;
   try {
     const Py_ssize_t count = PyList_GET_SIZE(list);
+    struct Seen { c10::TensorImpl* p; void *at, *grad; uint64_t order; };
+    std::vector<Seen> seen(count);
+    Py_ssize_t grads = 0;
     for (Py_ssize_t i = 0; i < count; ++i) {
       PyObject* o = PyList_GET_ITEM(list, i);
       const char* wrong = nullptr;
       if (!THPVariable_Check(o)) wrong = "is not a tensor";
       else {
         const at::Tensor& p = THPVariable_Unpack(o);
+        Seen& s = seen[i];
         if (p.layout() != at::kStrided || p.device().index() != device || p.device().is_cuda() != (device >= 0)) wrong = "has left the optimizer's device";
         else if (p.numel() != want[i].n || code_of(p.scalar_type()) != want[i].dt) wrong = "has another size or type than when the optimizer first ran";
         else if (!p.is_non_overlapping_and_dense() || p.is_neg()) wrong = "is not dense in memory";
         else if (p.is_inference()) wrong = "was made in inference mode: it has no version to count";
-        else if (orders[i] && orders[i] != order_of(p)) wrong = "has its elements in another order than when the optimizer first ran";
-        else if (const at::Tensor& g = p.grad(); g.defined()) {
-          if (g.layout() != at::kStrided) wrong = "has a sparse gradient";
-          else if (g.device() != p.device() || g.scalar_type() != p.scalar_type() || g.sizes() != p.sizes()) wrong = "has a gradient of another device, type or shape";
-          else (void)g.data_ptr();      // (throws where there is no memory behind it)
+        else if (s.order = order_of(p); orders[i] && orders[i] != s.order) wrong = "has its elements in another order than when the optimizer first ran";
+        else {
+          s.at = p.data_ptr();      // (throws where there is no memory behind it)
+          if (const at::Tensor& g = p.grad(); g.defined()) {
+            if (g.layout() != at::kStrided) wrong = "has a sparse gradient";
+            else if (g.device() != p.device() || g.scalar_type() != p.scalar_type() || g.sizes() != p.sizes()) wrong = "has a gradient of another device, type or shape";
+            else {
+              ++grads;
+              s.p = p.unsafeGetTensorImpl();
+              void* const at = g.data_ptr();
+              if (same_order(p, g)) s.grad = at;
+              else {
+                if (!other && !(other = PyList_New(0))) return nullptr;
+                PyObject* k = PyLong_FromSsize_t(i);
+                const int err = k ? PyList_Append(other, k) : -1;
+                Py_XDECREF(k);
+                if (err) { Py_DECREF(other); return nullptr; }
+              }
+            }
+          }
         }
-        if (!wrong) (void)p.data_ptr();
       }
-      if (wrong) return PyErr_Format(PyExc_ValueError, "parameter %zd %s", i, wrong);
-    }
-    Py_ssize_t grads = 0;
-    bool moved = false;
-    for (Py_ssize_t i = 0; i < count; ++i) {
-      const at::Tensor& p = THPVariable_Unpack(PyList_GET_ITEM(list, i));
-      const at::Tensor& g = p.grad();
-      out[i] = 0;
-      if (!g.defined()) continue;
-      ++grads;
-      if (same_order(p, g)) { out[i] = reinterpret_cast<uint64_t>(g.data_ptr()); continue; }
-      if (!other && !(other = PyList_New(0))) return nullptr;
-      PyObject* k = PyLong_FromSsize_t(i);
-      const int err = k ? PyList_Append(other, k) : -1;
-      Py_XDECREF(k);
-      if (err) { Py_DECREF(other); return nullptr; }
+      if (wrong) {
+        Py_XDECREF(other);
+        return PyErr_Format(PyExc_ValueError, "parameter %zd %s", i, wrong);
+      }
     }
     // nothing fails from here on
+    bool moved = false;
     for (Py_ssize_t i = 0; i < count; ++i) {
-      const at::Tensor& p = THPVariable_Unpack(PyList_GET_ITEM(list, i));
-      void* const at = p.data_ptr();
-      moved |= want[i].p != at;
-      want[i].p = at;
-      orders[i] = order_of(p);
-      if (update && p.grad().defined()) p.unsafeGetTensorImpl()->bump_version();      // the kernel writes it behind autograd's back: a stale saved tensor has to be noticed
+      const Seen& s = seen[i];
+      moved |= want[i].p != s.at;
+      want[i].p = s.at;
+      orders[i] = s.order;
+      out[i] = reinterpret_cast<uint64_t>(s.grad);
+      if (update && s.p) s.p->bump_version();      // the kernel writes it behind autograd's back: a stale saved tensor has to be noticed
     }
     PyObject* const flag = moved ? Py_True : Py_False;
     return other ? Py_BuildValue("nON", grads, flag, other) : Py_BuildValue("nOO", grads, flag, Py_None);
