@@ -344,6 +344,6 @@ def host_tensors():
         loader = importlib.machinery.ExtensionFileLoader("_host_tensors", path)
         host = importlib.util.module_from_spec(importlib.util.spec_from_loader("_host_tensors", loader))
         loader.exec_module(host)
-        host.bind(*(C.cast(f, c_void_p).value for f in (lib.mpmae_linear_i8, lib.mpmae_linear_i8_part_bytes, lib.mpmae_quant_i8)))
+        host.bind(*(C.cast(f, c_void_p).value for f in (lib.mpmae_linear_i8, lib.mpmae_linear_i8_part_bytes, lib.mpmae_quant_i8, lib.mpmae_adamw_multi)))
         _host = host
     return _host

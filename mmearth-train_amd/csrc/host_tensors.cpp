@@ -60,8 +60,10 @@ PyObject* gather(PyObject*, PyObject* args) {
   PyObject* other = nullptr;
   try {
     const Py_ssize_t count = PyList_GET_SIZE(list);
+    const c10::Device home(device >= 0 ? c10::DeviceType::CUDA : c10::DeviceType::CPU, (c10::DeviceIndex)device);
     struct Seen { c10::TensorImpl* p; void *at, *grad; uint64_t order; };
-    std::vector<Seen> seen(count);
+    static thread_local std::vector<Seen> seen;
+    seen.assign(count, Seen{});
     Py_ssize_t grads = 0;
     for (Py_ssize_t i = 0; i < count; ++i) {
       PyObject* o = PyList_GET_ITEM(list, i);
@@ -70,7 +72,7 @@ PyObject* gather(PyObject*, PyObject* args) {
       else {
         const at::Tensor& p = THPVariable_Unpack(o);
         Seen& s = seen[i];
-        if (p.layout() != at::kStrided || p.device().index() != device || p.device().is_cuda() != (device >= 0)) wrong = "has left the optimizer's device";
+        if (p.layout() != at::kStrided || p.device() != home) wrong = "has left the optimizer's device";
         else if (p.numel() != want[i].n || code_of(p.scalar_type()) != want[i].dt) wrong = "has another size or type than when the optimizer first ran";
         else if (!p.is_non_overlapping_and_dense() || p.is_neg()) wrong = "is not dense in memory";
         else if (p.is_inference()) wrong = "was made in inference mode: it has no version to count";
@@ -79,7 +81,7 @@ PyObject* gather(PyObject*, PyObject* args) {
           s.at = p.data_ptr();      // (throws where there is no memory behind it)
           if (const at::Tensor& g = p.grad(); g.defined()) {
             if (g.layout() != at::kStrided) wrong = "has a sparse gradient";
-            else if (g.device() != p.device() || g.scalar_type() != p.scalar_type() || g.sizes() != p.sizes()) wrong = "has a gradient of another device, type or shape";
+            else if (g.device() != home || g.scalar_type() != p.scalar_type() || g.sizes() != p.sizes()) wrong = "has a gradient of another device, type or shape";
             else {
               ++grads;
               s.p = p.unsafeGetTensorImpl();
@@ -142,6 +144,49 @@ PyObject* same_lists(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   return PyBool_FromLong(at == total);
 }
 
+using AdamwEntry = int (*)(const MpmaeAdamwArgs*, const void* const*, const double*, int, mpmae_stream_t);
+AdamwEntry adamw_entry = nullptr;          // of libmpmae_hip.so, from bind()
+
+// adamw(address of MpmaeAdamwArgs, address of the gradients' addresses, param_groups, device) -> 2 * hipError + whether the stream is being captured. The settings of
+// the groups, the stream and the launches of a step: through ctypes they take as long again as the launches.
+PyObject* adamw(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  if (nargs != 4 || !PyList_Check(args[2])) return PyErr_Format(PyExc_TypeError, "adamw(args, grads, param_groups, device)");
+  const auto* const a = static_cast<const MpmaeAdamwArgs*>(PyLong_AsVoidPtr(args[0]));
+  const auto* const grads = static_cast<const void* const*>(PyLong_AsVoidPtr(args[1]));
+  const long device = PyLong_AsLong(args[3]);
+  if (PyErr_Occurred()) return nullptr;
+  static PyObject* const keys[4] = {PyUnicode_InternFromString("lr"), PyUnicode_InternFromString("betas"), PyUnicode_InternFromString("eps"),
+                                    PyUnicode_InternFromString("weight_decay")};
+  const Py_ssize_t ngroups = PyList_GET_SIZE(args[2]);
+  std::vector<double> groups(5 * ngroups);
+  for (Py_ssize_t g = 0; g < ngroups; ++g) {
+    PyObject* const group = PyList_GET_ITEM(args[2], g);
+    PyObject* v[5];
+    for (int i = 0, at = 0; i < 4; ++i) {
+      PyObject* const x = PyDict_Check(group) ? PyDict_GetItemWithError(group, keys[i]) : nullptr;      // (borrowed)
+      if (!x) return PyErr_Occurred() ? nullptr : PyErr_Format(PyExc_KeyError, "a parameter group has no %U", keys[i]);
+      if (i != 1) { v[at++] = x; continue; }
+      if (!(PyTuple_Check(x) || PyList_Check(x)) || PySequence_Fast_GET_SIZE(x) != 2) return PyErr_Format(PyExc_ValueError, "betas are two numbers: %R", x);
+      v[at++] = PySequence_Fast_GET_ITEM(x, 0);
+      v[at++] = PySequence_Fast_GET_ITEM(x, 1);
+    }
+    if (THPVariable_Check(v[0])) return PyErr_Format(PyExc_ValueError, "lr is a number: a tensor would have to be read back on every step");
+    for (int i = 0; i < 5; ++i) {
+      groups[5 * g + i] = PyFloat_AsDouble(v[i]);
+      if (groups[5 * g + i] == -1.0 && PyErr_Occurred()) return nullptr;
+    }
+  }
+  TORCH_CHECK(adamw_entry, "the kernels are not loaded");
+  c10::OptionalDeviceGuard guard(c10::Device(c10::DeviceType::CUDA, (c10::DeviceIndex)device));
+  const hipStream_t stream = c10::hip::getCurrentHIPStream((c10::DeviceIndex)device).stream();
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  if (hipStreamIsCapturing(stream, &status) != hipSuccess) (void)hipGetLastError();
+  const int err = adamw_entry(a, grads, groups.data(), (int)ngroups, stream);
+  return PyLong_FromLong(2l * err + (status != hipStreamCaptureStatusNone));
+  END_HANDLE_TH_ERRORS
+}
+
 // ---- the int8 linear layer and its quantiser, as operators of torch's dispatcher (mpmae::linear_int8, mpmae::quantize_int8): a trace, a dispatch mode or a
 // functional transform sees the call. What they allocate is filled by this library, behind the dispatcher's back, so nothing above may take it for the result.
 using LinearEntry = int (*)(int, const MpmaeI8Args*, mpmae_stream_t);
@@ -152,8 +197,9 @@ PartBytes part_bytes = nullptr;
 QuantEntry quant_entry = nullptr;
 
 PyObject* bind(PyObject*, PyObject* args) {
-  unsigned long long linear, part, quant;
-  if (!PyArg_ParseTuple(args, "KKK", &linear, &part, &quant)) return nullptr;
+  unsigned long long linear, part, quant, adamw;
+  if (!PyArg_ParseTuple(args, "KKKK", &linear, &part, &quant, &adamw)) return nullptr;
+  adamw_entry = reinterpret_cast<AdamwEntry>(adamw);
   linear_entry = reinterpret_cast<LinearEntry>(linear);
   part_bytes = reinterpret_cast<PartBytes>(part);
   quant_entry = reinterpret_cast<QuantEntry>(quant);
@@ -283,6 +329,7 @@ TORCH_LIBRARY_IMPL(mpmae, Autograd, m) { m.impl("linear_int8", linear_autograd);
 PyMethodDef methods[] = {{"gather", gather, METH_VARARGS, "addresses of parameters and gradients"},
                          {"same_lists", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(same_lists)), METH_FASTCALL, "whether parameter lists are still the same"},
                          {"linear_i8", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(linear_i8)), METH_FASTCALL, "int8 linear layer"},
+                         {"adamw", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(adamw)), METH_FASTCALL, "one step"},
                          {"bind", bind, METH_VARARGS, "entry points of the kernel library"}, {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host_tensors", nullptr, -1, methods};
 

@@ -81,7 +81,7 @@ class _Plan:
         self.args = _lib.AdamwArgs(tensors=at(self.d_table), chunks=at(self.d_chunks), chunk_first=self.chunk_first.ctypes.data, steps=at(self.steps),
                                    hyper=at(self.hyper), partials=at(self.partials), norm_skip=at(self.norm_skip), m=at(self.m), v=at(self.v),
                                    ms=at(self.ms), vs=at(self.vs), max_norm=float(max_norm or 0.0), nt=nt, npartials=npart, bits=bits)
-        self.ref, self.stale = C.byref(self.args), False          # stale: parameters have moved and the device table does not know
+        self.at, self.stale = C.addressof(self.args), False          # stale: parameters have moved and the device table does not know
         self.captured = False                                     # a graph holds the addresses of these buffers
         self.table_at, self.grads_at, self.orders_at = self.table.ctypes.data, self.grads.ctypes.data, self.orders.ctypes.data
         _lib.host_tensors().gather(params, self.table_at, device.index, self.grads_at, self.orders_at, False)      # (holds them to the order that offsets go by)
@@ -275,18 +275,12 @@ class AdamW(torch.optim.Optimizer):
             p = plan.params[i]
             copies.append(torch.empty_like(p, memory_format=torch.preserve_format).copy_(p.grad))
             plan.grads[i] = copies[-1].data_ptr()
-        groups = []
-        for g in self.param_groups:
-            if isinstance(g["lr"], torch.Tensor):
-                raise ValueError("lr is a number: a tensor would have to be read back on every step")
-            groups += (g["lr"], *g["betas"], g["eps"], g["weight_decay"])
-        hyper = (C.c_double * len(groups))(*groups)
-        try:
-            plan.launch("adamw_multi", lambda stream: _lib.load().mpmae_adamw_multi(plan.ref, plan.grads_at, hyper, len(self.param_groups), stream))
-        except _lib.HipLibraryError:
+        done = _lib.host_tensors().adamw(plan.at, plan.grads_at, self.param_groups, plan.device.index)
+        plan.captured |= bool(done & 1)
+        if done > 1:
             for g in self.param_groups:                # (what the native call refuses, in words)
                 self._check_group(g)
-            raise
+            _lib.check(done >> 1, "adamw_multi")
         return loss
 
     # ---- checkpoints: torch.optim.AdamW's layout -------------------------------------------------------------------------------------------
