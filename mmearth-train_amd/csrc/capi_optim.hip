@@ -61,8 +61,10 @@ int mpmae_adamw_multi(const MpmaeAdamwArgs* a, const void* const* grads, const d
     const auto c = take(skip ? nl - 1 - l : l);
     const int nc = c.second - c.first;
     if (nc < 1) continue;
-    if (a->bits == 32)
-      LAUNCH(adamw32_kernel, dim3(nc), dim3(256), 0, S_(s), q, tensors, chunks + c.first, (const AdamwHyper*)a->hyper, (float*)a->m, (float*)a->v, skip);
+    if (a->bits == 32 && skip)
+      LAUNCH(adamw32_kernel<true>, dim3(nc), dim3(256), 0, S_(s), q, tensors, chunks + c.first, (const AdamwHyper*)a->hyper, (float*)a->m, (float*)a->v, skip);
+    else if (a->bits == 32)
+      LAUNCH(adamw32_kernel<false>, dim3(nc), dim3(256), 0, S_(s), q, tensors, chunks + c.first, (const AdamwHyper*)a->hyper, (float*)a->m, (float*)a->v, skip);
     else
       LAUNCH(adamw8_kernel, dim3(nc), dim3(256), 0, S_(s), q, tensors, chunks + c.first, (const AdamwHyper*)a->hyper, (uint8_t*)a->m, (uint8_t*)a->v,
              a->ms, a->vs, skip);
