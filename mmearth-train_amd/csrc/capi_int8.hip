@@ -53,7 +53,7 @@ static int i8_splits(int M, int N, int Kp) {
 }
 template <typename T>
 static void linear_i8(const MpmaeI8Args& a, hipStream_t st) {
-  // Up to 8 rows of a moderate length: one launch that quantises and multiplies (1 x 1024 -> 4096: 4.8 us; 7.2 us in two launches). A workgroup holds the rows in
+  // Up to 8 rows of a moderate length: one launch that quantises and multiplies (1 x 1024 -> 4096: 4.1 us; 7.2 us in two launches). A workgroup holds the rows in
   // its registers; longer ones go through a launch of their own.
   if (a.M <= 8 && i8_vectors(a.M, a.ldq) <= I8_KEPT && a.K >= 8) return skinny<T, true>(a, st);
   quant_rows((const T*)a.x, a.ldx, a.M, a.K, a.q, a.ldq, a.sx, st);

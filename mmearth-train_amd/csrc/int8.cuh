@@ -5,9 +5,10 @@
 // The integer sums are exact, so neither the order of k nor a split of it changes a result. A row that holds NaN or infinity has the scale NaN and
 // codes 0: its outputs are NaN, the other rows are untouched. Rows of codes are padded with zeros to a multiple of I8_KPAD bytes.
 //
-// Measured (bf16, bias; quantisation + product in us): 1 x 1024 -> 4096 4.3 in one launch; 8 x 2816 -> 1000 6.6 in one launch; 49 x 2816 -> 11264 3.6 + 9.5;
-// 50176 x 512 -> 2048 16 + 75 (1.4 PTOP/s: 27 % of the time in the matrix cores, output 205 MB); 12544 x 11264 -> 2816 81 + 335 (2.3 PTOP/s). The library's
-// int8 product reaches 2.4 PTOP/s at 16384^3 and takes 401 us for the last one, 120 us for the one before it, 21 us for 49 rows.
+// Measured (bf16, bias; quantisation + product in us, traced, after a hundred calls): 1 x 1024 -> 4096 4.1 in one launch; 8 x 2816 -> 1000 6.2 in one launch;
+// 49 x 2816 -> 11264 3.6 + 9.4; 50176 x 512 -> 2048 16 + 82 (94 a call untraced; 27 % of the time in the matrix cores, output 205 MB); 12544 x 11264 -> 2816 75 + 303
+// in whole rounds + 41 for the rest (2.3 PTOP/s). The library's int8 product reaches 2.4 PTOP/s at 16384^3 and takes 401 us for the last one, 120 us for
+// the one before it, 21 us for 49 rows.
 #pragma once
 #include "vec8.cuh"
 #include <type_traits>

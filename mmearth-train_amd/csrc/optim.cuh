@@ -11,9 +11,9 @@
 //
 // Everything is bound by memory: 3 * sizeof(p) + 16 bytes per element (fp32 moments), 3 * sizeof(p) + 4 + 1/16 (8 bits), + sizeof(p) for the norm, whose pass
 // over the gradients has to end before the first update. A large copy moves 4.8 TB/s on this card, a large sum reads 4.0.
-//   660 M parameters, bf16, fp32 moments: 2.75 ms, 5.3 TB/s.   88.7 M fp32 with a clip: norm 100 us (3.6 TB/s) + 430 us (5.8 TB/s of addressed bytes).
-//   660 M fp32, 8 bits: 1.94 ms, 5.5 TB/s.                     88.7 M bf16, 8 bits, with a clip: norm 56 us + 185 us (4.8 TB/s; vector units 90 % busy).
-//   3.7 M fp32 (144 tensors): 21 us (fp32 moments), 15 us (8 bits), next to 3 us for the step's records.
+//   660 M parameters, bf16, fp32 moments: 2.76 ms, 5.3 TB/s.   88.7 M fp32 with a clip: norm 101 us (3.5 TB/s) + 423 us (5.9 TB/s of addressed bytes).
+//   660 M fp32, 8 bits: 1.94 ms, 5.5 TB/s.                     88.7 M bf16, 8 bits, with a clip: norm 56 us + 156 us (5.7 TB/s; vector units nine tenths busy).
+//   3.7 M fp32 (144 tensors): 19 us (fp32 moments), 14 us (8 bits), next to 2.4 us for the step's records.
 // A workgroup takes one piece of 2048 elements of one tensor, a thread one vector of eight: 4096-element pieces were 4 % slower, and the piece list (8 bytes per
 // piece, made once) lets a launch cover tensors of one element and of 10^9 alike.
 #pragma once
