@@ -12,6 +12,7 @@
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/utils/object_ptr.h>
 #include <torch/library.h>
 #include <Python.h>
 #include <cstdint>
@@ -162,19 +163,20 @@ PyObject* adamw(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   std::vector<double> groups(5 * ngroups);
   for (Py_ssize_t g = 0; g < ngroups; ++g) {
     PyObject* const group = PyList_GET_ITEM(args[2], g);
-    PyObject* v[5];
-    for (int i = 0, at = 0; i < 4; ++i) {
+    double* out = groups.data() + 5 * g;
+    const auto number = [&](PyObject* x) { *out = PyFloat_AsDouble(x); return *out++ != -1.0 || !PyErr_Occurred(); };
+    for (int i = 0; i < 4; ++i) {
       PyObject* const x = PyDict_Check(group) ? PyDict_GetItemWithError(group, keys[i]) : nullptr;      // (borrowed)
       if (!x) return PyErr_Occurred() ? nullptr : PyErr_Format(PyExc_KeyError, "a parameter group has no %U", keys[i]);
-      if (i != 1) { v[at++] = x; continue; }
-      if (!(PyTuple_Check(x) || PyList_Check(x)) || PySequence_Fast_GET_SIZE(x) != 2) return PyErr_Format(PyExc_ValueError, "betas are two numbers: %R", x);
-      v[at++] = PySequence_Fast_GET_ITEM(x, 0);
-      v[at++] = PySequence_Fast_GET_ITEM(x, 1);
-    }
-    if (THPVariable_Check(v[0])) return PyErr_Format(PyExc_ValueError, "lr is a number: a tensor would have to be read back on every step");
-    for (int i = 0; i < 5; ++i) {
-      groups[5 * g + i] = PyFloat_AsDouble(v[i]);
-      if (groups[5 * g + i] == -1.0 && PyErr_Occurred()) return nullptr;
+      if (i == 0 && THPVariable_Check(x)) return PyErr_Format(PyExc_ValueError, "lr is a number: a tensor would have to be read back on every step");
+      if (i != 1) {
+        if (!number(x)) return nullptr;
+        continue;
+      }
+      const THPObjectPtr two(PySequence_Fast(x, "betas are two numbers"));
+      if (!two) return nullptr;
+      if (PySequence_Fast_GET_SIZE(two.get()) != 2) return PyErr_Format(PyExc_ValueError, "betas are two numbers: %R", x);
+      for (int j = 0; j < 2; ++j) if (!number(PySequence_Fast_GET_ITEM(two.get(), j))) return nullptr;
     }
   }
   TORCH_CHECK(adamw_entry, "the kernels are not loaded");

@@ -783,3 +783,37 @@ def test_settings_changed_to_impossible_ones_are_refused():
         assert torch.equal(keep, params[0].detach()) and opt.plan.steps.tolist() == [1]
     opt.step()
     assert opt.plan.steps.tolist() == [2]
+
+
+def test_settings_of_any_numeric_type():
+    """What a configuration or a scheduler puts into the groups: numpy numbers, betas as a list or an array; what is no number is refused with its own error."""
+    from mmearth_train_amd.optim import AdamW
+    params, twin = params_of([300], DT[:1], 29), params_of([300], DT[:1], 29)
+    a, b = AdamW(params, lr=1e-3, betas=(0.9, 0.99)), AdamW(twin, lr=1e-3, betas=(0.9, 0.99))
+    for ps in (params, twin):
+        grads_for(ps, 170)
+    for betas in ([0.9, 0.99], np.array([0.9, 0.99]), iter_twice(0.9, 0.99)):
+        a.param_groups[0].update(lr=np.float64(1e-3), betas=betas, weight_decay=np.float64(1e-2))
+        a.step(), b.step()
+        assert torch.equal(params[0], twin[0])
+    for key, value, error in (("betas", (0.9,), ValueError), ("betas", 0.9, TypeError), ("lr", "fast", TypeError), ("lr", torch.tensor(1e-3), ValueError), ("eps", None, TypeError)):
+        old = a.param_groups[0][key]
+        a.param_groups[0][key] = value
+        with pytest.raises(error):
+            a.step()
+        a.param_groups[0][key] = old
+    del a.param_groups[0]["eps"]
+    with pytest.raises(KeyError, match="eps"):
+        a.step()
+    assert a.plan.steps.tolist() == [3] and torch.equal(params[0], twin[0])
+
+
+def iter_twice(*numbers):
+    """A sequence that is neither a list nor a tuple."""
+    class Seq:
+        def __len__(self):
+            return len(numbers)
+
+        def __getitem__(self, i):
+            return numbers[i]
+    return Seq()
