@@ -321,7 +321,7 @@ class AdamW(torch.optim.Optimizer):
             self._check_group({**self.defaults, **{k: v for k, v in g.items() if k != "params"}})
         plan = self.plan
         ids = [i for g in groups for i in g["params"]]
-        entries = [state_dict["state"].get(i) for i in ids]
+        entries = [state_dict["state"].get(i) or None for i in ids]          # (an empty entry, as reading `state[p]` leaves one behind, is none)
         for (shape, _), st in zip(plan.shapes, entries):
             for key in ("exp_avg", "exp_avg_sq") if st is not None else ():
                 if not isinstance(st.get(key), torch.Tensor) or st[key].shape != shape or st[key].is_complex():

@@ -817,3 +817,17 @@ def iter_twice(*numbers):
         def __getitem__(self, i):
             return numbers[i]
     return Seq()
+
+
+def test_an_empty_entry_of_a_checkpoint_is_none():
+    """`optimizer.state[p]` on torch's own class makes one for a parameter that was never stepped."""
+    from mmearth_train_amd.optim import AdamW
+    params = params_of([30, 40], DT[:1], 30)
+    theirs = torch.optim.AdamW([torch.nn.Parameter(p.detach().clone()) for p in params])
+    p, q = theirs.param_groups[0]["params"]
+    p.grad = torch.ones_like(p)
+    theirs.step()
+    assert theirs.state[q] == {}
+    opt = AdamW(params)
+    opt.load_state_dict(theirs.state_dict())
+    assert opt.plan.steps.tolist() == [1, 0] and sorted(opt.state_dict()["state"]) == [0]
